@@ -31,6 +31,10 @@ extern "C" {
 #define MI_DTYPE_F16 1
 #define MI_DTYPE_F32 2
 
+/* what a paged cache's pages hold */
+#define MI_STORE_SAME 0       /* the activations' dtype */
+#define MI_STORE_E4M3 1       /* 8-bit floats (OCP e4m3) with scales */
+
 /* status codes */
 #define MI_OK 0
 #define MI_ERR_INVALID -1     /* bad pointer / shape / stride / alignment */
@@ -514,6 +518,97 @@ int32_t mi_lm_head(const void* x, int64_t x_sm, const void* norm_w, float eps,
 
 /* Partial-buffer entries per row that mi_lm_head's argmax needs (0 if m or n <= 0). */
 int64_t mi_lm_head_partials(int64_t m, int64_t n);
+
+/*
+ * A paged KV cache, as one layer's arrays:
+ *   k_pages    [num_pages, n_kv_heads, page_size, head_dim]
+ *   v_pages    [num_pages, n_kv_heads, head_dim, page_size]   (transposed)
+ *   scales     [num_pages, n_kv_heads, 2] fp32, of K and V; 8-bit pages only
+ *   page_table [batch, slots] int32 (row stride pt_sb): position p of row b lies
+ *              in page page_table[b][p / page_size] at offset p % page_size
+ * all contiguous and 16-byte aligned, page_size 16, 32, 64, 128 or 256, head_dim
+ * up to 256.  A table entry outside [0, num_pages) is no page: nothing is written
+ * to it, and its keys are not attended.  An 8-bit entry (store MI_STORE_E4M3)
+ * stands for its e4m3 value times its page's scale, a power of two.  No
+ * counterpart in the reference, whose cache is dense (src/kv_cache.py:4-57).
+ *
+ * mi_rope_paged_append: RoPE of xq into q_out (both or neither NULL) and of xk,
+ * and the append of xk and xv, in one launch.  Token s of row b is at position
+ * start[b] + s (start NULL: start_pos + s) and rotated by that row of cos / sin
+ * (nearest row outside [0, table_rows)); the first query_lens[b] tokens (NULL: all
+ * seq_len) that have a place are appended, every token of xq is rotated.  Rotation
+ * in fp32, products and sum rounded separately, K rounded once to what the pages
+ * hold.  An 8-bit page's scale is the least power of two >= 2^-120 that brings the
+ * call's largest finite entry of the page and head to 448 at most; a page that
+ * already holds earlier positions keeps at least its scale, and its earlier entries
+ * are rounded again to a larger one.  A value that is not finite is stored as NaN.
+ * Unit head_dim strides; rows of xq [batch, n_heads, seq_len, head_dim], xk and xv
+ * [batch, n_kv_heads, ..]; cdtype = dtype or fp32.  Rows whose newest page is the
+ * same page, or a position twice in a call, leave one of the writers' values.
+ * The paged form of mi_rope and mi_rope_kv_append (src/rope.py:94-119, :255-313).
+ */
+int32_t mi_rope_paged_append(
+    const void* xq, const void* xk, const void* xv, const void* cos, const void* sin,
+    void* q_out, void* k_pages, void* v_pages, float* scales, const int32_t* page_table,
+    int64_t start_pos, const int64_t* start, const int64_t* query_lens, int64_t table_rows,
+    int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t seq_len, int64_t head_dim,
+    int64_t num_pages, int64_t page_size, int64_t slots, int64_t xq_sb, int64_t xq_sh,
+    int64_t xq_ss, int64_t xk_sb, int64_t xk_sh, int64_t xk_ss, int64_t xv_sb, int64_t xv_sh,
+    int64_t xv_ss, int64_t qo_sb, int64_t qo_sh, int64_t qo_ss, int64_t pt_sb, int64_t c_ss,
+    int64_t s_ss, int32_t dtype, int32_t cdtype, int32_t store, void* stream);
+
+/*
+ * Attention of each row's newest tokens over its pages: query token s <
+ * query_lens[b] (NULL: seq_len) of row b sees the keys j < seq_lens[b] -
+ * query_lens[b] + s + 1, seq_lens[b] counting the keys with the query tokens'
+ * own.  out [batch, n_heads, seq_len, head_dim] in q's dtype, lse (optional fp32
+ * [batch, n_heads, seq_len], natural log); a query that sees no key, and the rows
+ * behind query_lens[b], give 0 and -inf.  Keys behind seq_lens[b] are not counted,
+ * whatever their memory holds.  Scores, softmax and sums are fp32.
+ * num_splits (1..256) key ranges per row; more than one needs `part`, batch *
+ * n_heads * seq_len * num_splits * (head_dim + 2) floats.  mi_paged_attn_splits
+ * gives the count to use for a shape on the current device.
+ * The paged form of mi_flash_decode (src/flash_decode.py:236-370) for one or
+ * several query tokens.
+ */
+int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t n_kv_heads,
+                             int64_t seq_len, int64_t head_dim, int64_t page_size,
+                             int64_t slots, int32_t dtype, int32_t store);
+int32_t mi_paged_attn(
+    const void* q, const void* k_pages, const void* v_pages, const float* scales,
+    const int32_t* page_table, const int64_t* seq_lens, const int64_t* query_lens, float* part,
+    int64_t part_elems, void* out, float* lse, int64_t batch, int64_t n_heads,
+    int64_t n_kv_heads, int64_t seq_len, int64_t head_dim, int64_t num_pages, int64_t page_size,
+    int64_t slots, int64_t num_splits, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t o_sb,
+    int64_t o_sh, int64_t o_ss, int64_t pt_sb, float sm_scale, int32_t dtype, int32_t store,
+    void* stream);
+
+/*
+ * Verification of drafted tokens.  p_i = softmax(target[b][i] / temperature), i <=
+ * drafts; q_i = softmax(draft[b][i] / temperature), or with draft NULL the point
+ * mass of the drafted token.  Draft i < draft_lens[b] (NULL: drafts) is accepted
+ * iff accept_u[b][i] * q_i(x_i) < p_i(x_i) and all before it were; accepted[b] is
+ * their number n.  tokens[b] = the accepted tokens, then one more, then -1: the
+ * least j with cumsum(w)[j] > sample_u[b] * sum(w), w = max(p_n - q_n, 0) where
+ * draft n was refused (p_n if that is zero everywhere), else w = p_n.  Temperature
+ * 0: draft i is accepted iff it is the first largest logit of target[b][i], the
+ * next token is that of row n, and draft, accept_u and sample_u are not read.
+ * Shares and sums are fp64.  A NaN logit counts as -inf, +inf as the largest finite
+ * value; a row without mass refuses its draft and gives the token -1.  A drafted
+ * token outside [0, vocab) is refused.  target [batch, drafts + 1, vocab], draft
+ * [batch, drafts, vocab] (unit vocab stride), drafted and accept_u [batch, drafts],
+ * sample_u [batch], tokens [batch, drafts + 1] and accepted [batch] contiguous.
+ * drafts 1..128; workspace of mi_verify_drafts_workspace bytes, 8-byte aligned.
+ * Beside mi_lm_head's greedy argmax; the reference draws one token at a time on
+ * the host (src/sampler.py:4-33).
+ */
+int64_t mi_verify_drafts_workspace(int64_t batch, int64_t drafts, int64_t vocab);
+int32_t mi_verify_drafts(
+    const void* target, const void* draft, const int64_t* drafted, const float* accept_u,
+    const float* sample_u, const int64_t* draft_lens, int64_t* tokens, int64_t* accepted,
+    void* workspace, int64_t workspace_bytes, int64_t batch, int64_t drafts, int64_t vocab,
+    int64_t t_sb, int64_t t_ss, int64_t d_sb, int64_t d_ss, int64_t x_sb, int64_t x_ss,
+    int64_t u_sb, int64_t u_ss, double temperature, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,6 +19,8 @@ LIB_PATH = Path(os.environ.get("MIATTN_LIB", _PKG_ROOT / "libmiattn.so"))
 MI_DTYPE_BF16 = 0
 MI_DTYPE_F16 = 1
 MI_DTYPE_F32 = 2
+MI_STORE_SAME = 0
+MI_STORE_E4M3 = 1
 MI_OK = 0
 MI_ERR_INVALID = -1
 MI_ERR_UNSUPPORTED = -2
@@ -32,6 +34,7 @@ _DTYPE_CODES = {
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _ptr = ctypes.c_void_p
 
 # name -> (restype, [argtypes]).  Must mirror include/miattn.h exactly.
@@ -204,6 +207,40 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i64, _i64, _i64, _i32, _ptr,          # m n k dtype stream
     ]),
     "mi_lm_head_partials": (_i64, [_i64, _i64]),
+    "mi_rope_paged_append": (_i32, [
+        _ptr, _ptr, _ptr, _ptr, _ptr,          # xq xk xv cos sin
+        _ptr, _ptr, _ptr, _ptr, _ptr,          # q_out k_pages v_pages scales page_table
+        _i64, _ptr, _ptr, _i64,                # start_pos start query_lens table_rows
+        _i64, _i64, _i64, _i64, _i64,          # B Hq Hkv S D
+        _i64, _i64, _i64,                      # num_pages page_size slots
+        _i64, _i64, _i64,                      # xq strides (b, h, s)
+        _i64, _i64, _i64,                      # xk strides
+        _i64, _i64, _i64,                      # xv strides
+        _i64, _i64, _i64,                      # q_out strides
+        _i64, _i64, _i64,                      # page table, cos, sin row strides
+        _i32, _i32, _i32, _ptr,                # dtype cdtype store stream
+    ]),
+    "mi_paged_attn_splits": (_i64, [_i64] * 7 + [_i32, _i32]),
+    "mi_paged_attn": (_i32, [
+        _ptr, _ptr, _ptr, _ptr,                # q k_pages v_pages scales
+        _ptr, _ptr, _ptr, _ptr, _i64,          # page_table seq_lens query_lens part part_elems
+        _ptr, _ptr,                            # out lse
+        _i64, _i64, _i64, _i64, _i64,          # B Hq Hkv S D
+        _i64, _i64, _i64, _i64,                # num_pages page_size slots splits
+        _i64, _i64, _i64,                      # q strides (b, h, s)
+        _i64, _i64, _i64,                      # out strides
+        _i64,                                  # page table row stride
+        _f32, _i32, _i32, _ptr,                # sm_scale dtype store stream
+    ]),
+    "mi_verify_drafts_workspace": (_i64, [_i64, _i64, _i64]),
+    "mi_verify_drafts": (_i32, [
+        _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,    # target draft drafted accept_u sample_u draft_lens
+        _ptr, _ptr, _ptr, _i64,                # tokens accepted workspace workspace_bytes
+        _i64, _i64, _i64,                      # B drafts vocab
+        _i64, _i64, _i64, _i64,                # target, draft strides (b, row)
+        _i64, _i64, _i64, _i64,                # drafted, accept_u strides (b, draft)
+        _f64, _i32, _ptr,                      # temperature dtype stream
+    ]),
 }
 
 _lock = threading.Lock()
@@ -268,6 +305,28 @@ def stream_of(t: torch.Tensor) -> int:
     if index < 0:
         raise ValueError(f"needs a CUDA tensor, got one on {t.device}")
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+class _Here:
+    """A context that changes nothing (the tensors are on the current device)."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which t's device is the current one, for launches and for the
+    library's questions about the current device."""
+    index = t.get_device()
+    if index < 0 or index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(index)
 
 
 _ARRIVE: dict[tuple[int, int], int | None] = {}

@@ -1,0 +1,299 @@
+"""Paged KV cache, the append to it and the attention over it.
+
+The dense ``KVCache`` (src/kv_cache.py) reserves max_batch_size x max_seq_len
+slots and appends every row at one position.  ``PagedKVCache`` holds pages of
+``page_size`` tokens that any sequence may use; a page table [batch, slots]
+(int32, on the device) names each row's pages, and every row has its own length:
+
+  rope_and_paged_update   RoPE of q and k at each row's own positions, and the
+                          append of k and v (mi_rope_paged_append, one launch)
+  paged_flash_attention   causal attention of a row's newest tokens, one or many,
+                          over all its keys (mi_paged_attn)
+
+Pages hold the activations' dtype or, with ``kv_dtype=torch.float8_e4m3fn``, 8-bit
+floats with a power-of-two scale for each page, KV head and K / V.  V pages are
+transposed ([head_dim, page_size]): the attention's matrix instructions take V in
+that order straight from memory.
+
+Everything that varies while serving (lengths, counts, the table) is read on the
+device, so a captured step stays valid for other values of them.  A table entry
+that is no page of the cache takes no write and gives no key.  The paged cache has
+no counterpart in the reference, whose cache is dense (src/kv_cache.py:4-57).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .config import ModelArgs
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+class PagedKVCache:
+    """k [n_layers, num_pages, n_kv_heads, page_size, head_dim], v [n_layers,
+    num_pages, n_kv_heads, head_dim, page_size] and, for 8-bit pages, scales
+    [n_layers, num_pages, n_kv_heads, 2] (fp32; of K and V)."""
+
+    def __init__(self, args: ModelArgs, num_pages: int, page_size: int = 64,
+                 dtype: torch.dtype | None = None, *, kv_dtype: torch.dtype | None = None):
+        dtype = dtype if dtype is not None else torch.get_default_dtype()
+        kv_dtype = kv_dtype if kv_dtype is not None else dtype
+        d = args.dim // args.n_heads
+        shape = (args.n_layers, num_pages, args.n_kv_heads)
+        _check_pages(dtype, kv_dtype, num_pages, page_size, d)
+        k = torch.zeros((*shape, page_size, d), device=args.device, dtype=kv_dtype)
+        v = torch.zeros((*shape, d, page_size), device=args.device, dtype=kv_dtype)
+        scales = None
+        if kv_dtype != dtype:
+            scales = torch.zeros((*shape, 2), device=args.device, dtype=torch.float32)
+        self._set(k, v, scales, dtype)
+
+    @classmethod
+    def from_pages(cls, k: torch.Tensor, v: torch.Tensor, scales: torch.Tensor | None = None, *,
+                   dtype: torch.dtype | None = None) -> "PagedKVCache":
+        """A cache over existing pages (not copied): k [n_layers, num_pages, n_kv_heads,
+        page_size, head_dim] or one layer's [num_pages, ..], v the same transposed, scales
+        for 8-bit pages; ``dtype`` is the activations' (default: k's)."""
+        dtype = dtype if dtype is not None else k.dtype
+        if k.dim() == 4:
+            k, v = k[None], v[None] if v.dim() == 4 else v
+            scales = scales[None] if scales is not None and scales.dim() == 3 else scales
+        if k.dim() != 5 or v.shape != (*k.shape[:3], k.shape[4], k.shape[3]):
+            raise ValueError(f"PagedKVCache: k pages {tuple(k.shape)} and transposed v pages "
+                             f"{tuple(v.shape)} do not match")
+        if v.dtype != k.dtype or v.device != k.device:
+            raise TypeError("PagedKVCache: k and v must share a dtype and a device")
+        _check_pages(dtype, k.dtype, k.shape[1], k.shape[3], k.shape[4])
+        if (scales is None) != (k.dtype == dtype):
+            raise ValueError("PagedKVCache: 8-bit pages, and only they, have scales")
+        if scales is not None and (scales.shape != (*k.shape[:3], 2)
+                                   or scales.dtype != torch.float32
+                                   or scales.device != k.device):
+            raise ValueError(f"PagedKVCache: scales must be fp32 {(*k.shape[:3], 2)} on {k.device}")
+        for t in (k, v, scales):
+            if t is not None and not t.is_contiguous():
+                raise ValueError("PagedKVCache: pages and scales must be contiguous")
+        self = cls.__new__(cls)
+        self._set(k, v, scales, dtype)
+        return self
+
+    def _set(self, k, v, scales, dtype):
+        self.k, self.v, self.scales, self.dtype = k, v, scales, dtype
+        self.n_layers, self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self.kv_dtype = k.dtype
+        self.store = _lib.MI_STORE_SAME if scales is None else _lib.MI_STORE_E4M3
+
+    def reset(self):
+        """Empty pages (zeros).  Not needed before a page is used again: its first
+        append starts it anew."""
+        self.k.zero_()
+        self.v.zero_()
+        if self.scales is not None:
+            self.scales.zero_()
+
+    def _layer(self, layer_idx: int, what: str):
+        """Addresses of a layer's k, v and scales."""
+        n = self.n_layers
+        if not -n <= layer_idx < n:
+            raise ValueError(f"{what}: layer_idx {layer_idx} out of range for a cache of {n} layers")
+        i = layer_idx % n
+        k, v, s = self.k, self.v, self.scales
+        if not (k.is_cuda and v.is_cuda):
+            raise ValueError(f"{what} requires CUDA tensors")
+        return (k.data_ptr() + i * k.stride(0) * k.element_size(),
+                v.data_ptr() + i * v.stride(0) * v.element_size(),
+                None if s is None else s.data_ptr() + 4 * i * s.stride(0))
+
+
+def _check_pages(dtype, kv_dtype, num_pages, page_size, head_dim):
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"PagedKVCache: unsupported dtype {dtype}; expected bfloat16, float16 or "
+                        "float32")
+    if kv_dtype not in (dtype, torch.float8_e4m3fn):
+        raise TypeError(f"PagedKVCache: pages hold {dtype} or float8_e4m3fn, not {kv_dtype}")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"PagedKVCache: page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if num_pages < 1:
+        raise ValueError(f"PagedKVCache: num_pages must be positive, got {num_pages}")
+    if head_dim % 2 != 0 or not 2 <= head_dim <= 256:
+        raise ValueError(f"PagedKVCache: head_dim must be even and at most 256, got {head_dim}")
+
+
+def _per_row(t, batch: int, device, name: str, what: str):
+    """A device int64 [batch] tensor of row lengths or positions (None stays None)."""
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != batch:
+        raise ValueError(f"{what}: {name} must have shape ({batch},), got {tuple(t.shape)}")
+    if t.dtype != torch.int64 or t.device != device or t.stride(0) != 1:
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise TypeError(f"{what}: {name} must hold integers, got {t.dtype}")
+        t = t.to(device=device, dtype=torch.int64).contiguous()
+    return t
+
+
+def _table(page_table, batch: int, device, what: str):
+    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1:
+        raise ValueError(f"{what}: page_table must have shape ({batch}, slots), got "
+                         f"{tuple(page_table.shape)}")
+    if page_table.dtype != torch.int32:
+        raise TypeError(f"{what}: page_table must have dtype torch.int32, got {page_table.dtype}")
+    if page_table.device != device:
+        raise ValueError(f"{what}: page_table must be on {device}, got {page_table.device}")
+    return page_table if page_table.stride(1) == 1 else page_table.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with unit head_dim stride."""
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _check_heads(q, cache, n_kv_heads, what):
+    if q.shape[1] % n_kv_heads != 0:
+        raise ValueError(f"query heads ({q.shape[1]}) must be divisible by KV heads ({n_kv_heads})")
+    if q.dtype != cache.dtype:
+        raise TypeError(f"{what}: q dtype {q.dtype} must match the cache's activations "
+                        f"{cache.dtype}")
+
+
+def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer_idx: int,
+                          page_table, start_pos, *, query_lens=None, xq=None):
+    """RoPE of xk (and xq) and the append of xk, xv to the rows' pages.
+
+    xk, xv: [B, n_kv_heads, S, head_dim]; xq [B, n_heads, S, head_dim] or None.
+    Token s of row b is at position start_pos[b] + s (start_pos: device int64 [B],
+    or an int for all rows) and takes that row of the full tables rope_cos /
+    rope_sin [positions, head_dim // 2] (in xk's dtype or fp32; the nearest row
+    outside them).  With ``query_lens`` (device int64 [B]) only a row's first
+    query_lens[b] tokens are appended.  Positions behind the table's slots, before 0 or
+    in slots without a page are not written.
+
+    Returns the rotated xq (with xq's strides), or None.
+    """
+    what = "rope_and_paged_update"
+    if xk.dim() != 4 or xv.shape != xk.shape:
+        raise ValueError(f"xk and xv shapes must match, got {tuple(xk.shape)} and {tuple(xv.shape)}")
+    B, Hkv, S, D = xk.shape
+    dev = xk.device
+    if Hkv != cache.n_kv_heads or D != cache.head_dim:
+        raise ValueError(f"xk/xv shape {tuple(xk.shape)} does not fit a cache of "
+                         f"{cache.n_kv_heads} heads of {cache.head_dim}")
+    if xk.dtype != cache.dtype or xv.dtype != cache.dtype:
+        raise TypeError(f"xk/xv dtype {xk.dtype} must match the cache's activations {cache.dtype}")
+    H = Hkv
+    if xq is not None:
+        if xq.dim() != 4 or xq.shape[0] != B or xq.shape[2] != S or xq.shape[3] != D:
+            raise ValueError(f"xq shape {tuple(xq.shape)} does not match xk {tuple(xk.shape)}")
+        _check_heads(xq, cache, Hkv, what)
+        H = xq.shape[1]
+    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or rope_cos.shape[1] < D // 2:
+        raise ValueError(f"{what}: cos/sin must be 2-D [positions, head_dim // 2 = {D // 2}], got "
+                         f"{tuple(rope_cos.shape)} and {tuple(rope_sin.shape)}")
+    if rope_cos.dtype != rope_sin.dtype or rope_cos.dtype not in (xk.dtype, torch.float32):
+        raise TypeError(f"{what}: cos/sin must have dtype {xk.dtype} or float32, got "
+                        f"{rope_cos.dtype} and {rope_sin.dtype}")
+    kp, vp, sp = cache._layer(layer_idx, what)
+    for t in (xk, xv, rope_cos, rope_sin, cache.k, *(() if xq is None else (xq,))):
+        if not t.is_cuda:
+            raise ValueError(f"{what} requires CUDA tensors")
+        if t.device != dev:
+            raise ValueError(f"{what}: all tensors must be on {dev}, got one on {t.device}")
+    page_table = _table(page_table, B, dev, what)
+    first, start = 0, None
+    if isinstance(start_pos, torch.Tensor):
+        start = _per_row(start_pos, B, dev, "start_pos", what)
+    else:
+        first = int(start_pos)
+    query_lens = _per_row(query_lens, B, dev, "query_lens", what)
+    xk, xv = _rows(xk), _rows(xv)
+    if rope_cos.stride(1) != 1 or rope_sin.stride(1) != 1:
+        rope_cos, rope_sin = rope_cos.contiguous(), rope_sin.contiguous()
+    out = dst = qs = None
+    q_strides = o_strides = (0, 0, 0)
+    if xq is not None:
+        out = torch.empty_like(xq)
+        qs = _rows(xq)
+        dst = out if out.stride(3) == 1 else torch.empty(xq.shape, dtype=xq.dtype, device=dev)
+        q_strides, o_strides = qs.stride()[:3], dst.stride()[:3]
+    if B == 0 or S == 0:
+        return out
+    with _lib.on_device_of(xk):
+        st = _lib.load().mi_rope_paged_append(
+            _lib.ptr(qs), xk.data_ptr(), xv.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
+            _lib.ptr(dst), kp, vp, sp, page_table.data_ptr(), first, _lib.ptr(start),
+            _lib.ptr(query_lens), rope_cos.shape[0], B, H, Hkv, S, D, cache.num_pages,
+            cache.page_size, page_table.shape[1], *q_strides, *xk.stride()[:3],
+            *xv.stride()[:3], *o_strides, page_table.stride(0), rope_cos.stride(0),
+            rope_sin.stride(0), _lib.dtype_code(xk.dtype), _lib.dtype_code(rope_cos.dtype),
+            cache.store, _lib.stream_of(xk))
+    _lib.check(st, what)
+    if dst is not out:
+        out.copy_(dst)
+    return out
+
+
+def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, seq_lens, *,
+                          query_lens=None, num_splits: int | None = None,
+                          return_lse: bool = False, sm_scale: float | None = None):
+    """Causal attention of each row's newest tokens over the row's pages.
+
+    q: [B, n_heads, S, head_dim]; seq_lens (device int64 [B]) counts the row's keys,
+    those of its query tokens (already appended) among them.  The first
+    query_lens[b] of the S tokens (default: all) are row b's newest: token s sees
+    keys j < seq_lens[b] - query_lens[b] + s + 1.  Tokens behind query_lens[b], and a
+    token that sees no key, give 0.  out has q's strides; with ``return_lse`` also
+    the fp32 log-sum-exp [B, n_heads, S] of the scaled scores (-inf for those).
+    ``num_splits``: key ranges per row (default: chosen from the CU count).
+    """
+    what = "paged_flash_attention"
+    if q.dim() != 4:
+        raise ValueError("q must be a rank-4 tensor")
+    B, H, S, D = q.shape
+    dev = q.device
+    if D != cache.head_dim:
+        raise ValueError(f"q head_dim {D} does not fit a cache of head_dim {cache.head_dim}")
+    _check_heads(q, cache, cache.n_kv_heads, what)
+    if not q.is_cuda:
+        raise ValueError(f"{what} requires CUDA tensors")
+    kp, vp, sp = cache._layer(layer_idx, what)
+    if cache.k.device != dev:
+        raise ValueError(f"{what}: q is on {dev}, the cache on {cache.k.device}")
+    page_table = _table(page_table, B, dev, what)
+    if seq_lens is None:
+        raise ValueError(f"{what}: seq_lens must be given")
+    seq_lens = _per_row(seq_lens, B, dev, "seq_lens", what)
+    query_lens = _per_row(query_lens, B, dev, "query_lens", what)
+    if num_splits is not None and not 1 <= int(num_splits) <= 256:
+        raise ValueError(f"num_splits must be 1..256, got {num_splits}")
+    slots = page_table.shape[1]
+    code = _lib.dtype_code(q.dtype)
+    out = torch.empty_like(q)
+    lse = torch.empty((B, H, S), device=dev, dtype=torch.float32) if return_lse else None
+    if B == 0 or S == 0:
+        return (out, lse) if return_lse else out
+    lib = _lib.load()
+    qs = _rows(q)
+    dst = out if out.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    with _lib.on_device_of(q):
+        if num_splits is None:
+            num_splits = lib.mi_paged_attn_splits(B, H, cache.n_kv_heads, S, D, cache.page_size,
+                                                  slots, code, cache.store)
+        num_splits = int(num_splits)
+        part, n = None, 0
+        if num_splits > 1:
+            n = B * H * S * num_splits * (D + 2)
+            part = torch.empty(n, device=dev, dtype=torch.float32)
+        st = lib.mi_paged_attn(
+            qs.data_ptr(), kp, vp, sp, page_table.data_ptr(), seq_lens.data_ptr(),
+            _lib.ptr(query_lens), _lib.ptr(part), n, dst.data_ptr(), _lib.ptr(lse), B, H,
+            cache.n_kv_heads, S, D, cache.num_pages, cache.page_size, slots, num_splits,
+            *qs.stride()[:3], *dst.stride()[:3], page_table.stride(0), scale, code, cache.store,
+            _lib.stream_of(q))
+    _lib.check(st, what)
+    if dst is not out:
+        out.copy_(dst)
+    return (out, lse) if return_lse else out
