@@ -10,6 +10,9 @@
 // time: the lane's key against q from LDS, the softmax across the wave, then a lane
 // per dim over the transposed V.  bf16 and fp16 at head_dims that are multiples of
 // 64 run on the matrix cores instead (paged_attn_mfma.hpp).
+#include <initializer_list>
+#include <type_traits>
+
 #include "paged_attn_kernels.hpp"
 
 namespace mi {
@@ -218,8 +221,22 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 namespace {
 
 template <typename T>
-int32_t launch_attn(const PagedAttnArgs& a, bool e8, hipStream_t st) {
+int32_t launch_attn(const PagedAttnArgs& a, const PagedPlan& plan, bool e8, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Hq * a.S, blocks = rows * a.splits;
+  if constexpr (sizeof(T) == 2) {
+    if (plan.mfma) {
+      const int64_t x = (int64_t)a.B * a.Hkv * a.splits;
+      if (x > INT32_MAX || plan.tiles > 65535) {
+        set_last_error("paged_attn: too many rows and splits for one call");
+        return MI_ERR_UNSUPPORTED;
+      }
+      paged_attn_mfma_launch(a, plan, std::is_same<T, bf16_t>::value ? MI_DTYPE_BF16 : MI_DTYPE_F16,
+                             e8, st);
+      if (a.splits > 1)
+        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+      return MI_OK;
+    }
+  }
   if (blocks > INT32_MAX) {
     set_last_error("paged_attn: too many rows and splits for one call");
     return MI_ERR_UNSUPPORTED;
@@ -245,9 +262,11 @@ extern "C" int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t 
       page_size <= 0 || slots > INT32_MAX / page_size)
     return 1;
   const int64_t units = (slots * page_size + 63) / 64;
-  const int64_t blocks = batch * n_heads * seq_len;
-  // 8 blocks of 4 waves a compute unit, of 4 units of 64 keys or more each
-  int64_t s = (8 * (int64_t)device_cu_count() + blocks - 1) / blocks;
+  const PagedPlan plan = paged_plan(n_heads, n_kv_heads, seq_len, head_dim, dtype);
+  const int64_t blocks = plan.mfma ? batch * n_kv_heads * plan.tiles : batch * n_heads * seq_len;
+  // blocks of 4 waves a compute unit, of 4 units of 64 keys or more each
+  const int64_t want = (plan.mfma ? 2 : 8) * (int64_t)device_cu_count();
+  int64_t s = want / blocks;
   if (s > (units + 3) / 4) s = (units + 3) / 4;
   return s < 1 ? 1 : (s > 256 ? 256 : s);
 }
@@ -302,14 +321,23 @@ extern "C" int32_t mi_paged_attn(
   a.slots = (int32_t)slots; a.splits = (int32_t)num_splits;
   a.scale_log2 = sm_scale * kLog2e;
   const bool e8 = store == MI_STORE_E4M3;
+  const PagedPlan plan = paged_plan(n_heads, n_kv_heads, seq_len, head_dim, dtype);
+  const int64_t es = dtype == MI_DTYPE_F32 ? 4 : 2;
+  auto rows_of = [&](const void* p, int64_t n, std::initializer_list<int64_t> strides) {
+    bool ok = (uintptr_t)p % n == 0;
+    for (int64_t s : strides) ok = ok && (s * es) % n == 0;
+    return ok;
+  };
+  a.q_vec = rows_of(q, 16, {q_sb, q_sh, q_ss});
+  a.o_vec = rows_of(out, 8, {o_sb, o_sh, o_ss});
   hipStream_t st = (hipStream_t)stream;
   int32_t rc;
   if (dtype == MI_DTYPE_BF16)
-    rc = launch_attn<bf16_t>(a, e8, st);
+    rc = launch_attn<bf16_t>(a, plan, e8, st);
   else if (dtype == MI_DTYPE_F16)
-    rc = launch_attn<f16_t>(a, e8, st);
+    rc = launch_attn<f16_t>(a, plan, e8, st);
   else
-    rc = launch_attn<float>(a, e8, st);
+    rc = launch_attn<float>(a, plan, e8, st);
   if (rc != MI_OK) return rc;
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

@@ -23,7 +23,20 @@ struct PagedAttnArgs {
   int64_t t_sb, num_pages;
   int32_t B, Hq, Hkv, group, S, D, P, p_shift, slots, splits;
   float scale_log2;
+  int32_t q_vec, o_vec;     // q rows 16-byte, out rows 8-byte aligned
 };
+
+// How a call's rows are laid on blocks.
+struct PagedPlan {
+  bool mfma;       // the matrix-core kernel, else one block a (row, split)
+  int r;           // 16-row tiles of a wave
+  bool rows;       // a block's waves take different rows (else different keys)
+  int64_t tiles;   // blocks along the rows of a KV head
+};
+PagedPlan paged_plan(int64_t n_heads, int64_t n_kv_heads, int64_t seq_len, int64_t head_dim,
+                     int32_t dtype);
+void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32_t dtype, bool e8,
+                            hipStream_t st);
 
 // Row b's keys as its query tokens see them: token s sees keys [0, vis(s)).
 struct RowKeys {
