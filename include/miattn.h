@@ -565,15 +565,21 @@ int32_t mi_rope_paged_append(
  * [batch, n_heads, seq_len], natural log); a query that sees no key, and the rows
  * behind query_lens[b], give 0 and -inf.  Keys behind seq_lens[b] are not counted,
  * whatever their memory holds.  Scores, softmax and sums are fp32.
- * num_splits (1..256) key ranges per row; more than one needs `part`, batch *
- * n_heads * seq_len * num_splits * (head_dim + 2) floats.  mi_paged_attn_splits
- * gives the count to use for a shape on the current device.
+ * num_splits: 1, a row's keys are not divided (one launch); 2..
+ * MI_PAGED_ATTN_MAX_SPLITS, the keys of a KV head, those of all rows together, are
+ * divided into so many parts, which needs `part`, 16-byte aligned, of
+ * mi_paged_attn_workspace floats (0: none).
+ * mi_paged_attn_splits gives the count to use for a shape on the current device.
  * The paged form of mi_flash_decode (src/flash_decode.py:236-370) for one or
  * several query tokens.
  */
+#define MI_PAGED_ATTN_MAX_SPLITS 65536
 int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t n_kv_heads,
                              int64_t seq_len, int64_t head_dim, int64_t page_size,
                              int64_t slots, int32_t dtype, int32_t store);
+int64_t mi_paged_attn_workspace(int64_t batch, int64_t n_heads, int64_t n_kv_heads,
+                                int64_t seq_len, int64_t head_dim, int64_t num_splits,
+                                int32_t dtype);
 int32_t mi_paged_attn(
     const void* q, const void* k_pages, const void* v_pages, const float* scales,
     const int32_t* page_table, const int64_t* seq_lens, const int64_t* query_lens, float* part,

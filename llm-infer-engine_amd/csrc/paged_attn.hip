@@ -8,10 +8,8 @@
 // paged_attn_kernel (below) computes it in fp32 for any type and head_dim up to
 // 256, one block for each (row, head, token, key range), a wave taking 64 keys at a
 // time: the lane's key against q from LDS, the softmax across the wave, then a lane
-// per dim over the transposed V.  bf16 and fp16 at head_dims that are multiples of
-// 64 run on the matrix cores instead (paged_attn_mfma.hpp).
+// per dim over the transposed V.  bf16 and fp16 at head_dim 64, 128 and 256 run on the matrix cores instead (paged_attn_mfma.hpp).
 #include <initializer_list>
-#include <type_traits>
 
 #include "paged_attn_kernels.hpp"
 
@@ -221,22 +219,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 namespace {
 
 template <typename T>
-int32_t launch_attn(const PagedAttnArgs& a, const PagedPlan& plan, bool e8, hipStream_t st) {
+int32_t launch_attn(const PagedAttnArgs& a, bool e8, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Hq * a.S, blocks = rows * a.splits;
-  if constexpr (sizeof(T) == 2) {
-    if (plan.mfma) {
-      const int64_t x = (int64_t)a.B * a.Hkv * a.splits;
-      if (x > INT32_MAX || plan.tiles > 65535) {
-        set_last_error("paged_attn: too many rows and splits for one call");
-        return MI_ERR_UNSUPPORTED;
-      }
-      paged_attn_mfma_launch(a, plan, std::is_same<T, bf16_t>::value ? MI_DTYPE_BF16 : MI_DTYPE_F16,
-                             e8, st);
-      if (a.splits > 1)
-        hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-      return MI_OK;
-    }
-  }
   if (blocks > INT32_MAX) {
     set_last_error("paged_attn: too many rows and splits for one call");
     return MI_ERR_UNSUPPORTED;
@@ -255,20 +239,42 @@ int32_t launch_attn(const PagedAttnArgs& a, const PagedPlan& plan, bool e8, hipS
 
 using namespace mi;
 
+// num_splits counts parts of a KV head's keys over all rows; the kernel of any type divides
+// each row's keys alike.
+static int64_t ranges_per_row(int64_t num_splits, int64_t batch) {
+  const int64_t n = num_splits / batch;
+  return n < 1 ? 1 : (n > 256 ? 256 : n);
+}
+
 extern "C" int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t n_kv_heads,
                                         int64_t seq_len, int64_t head_dim, int64_t page_size,
                                         int64_t slots, int32_t dtype, int32_t store) {
   if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || seq_len <= 0 || slots <= 0 ||
-      page_size <= 0 || slots > INT32_MAX / page_size)
+      page_size <= 0 || slots > INT32_MAX / page_size || batch > (1 << 24) ||
+      n_heads > (1 << 16) || n_heads % n_kv_heads != 0 || seq_len > (1 << 24))
     return 1;
   const int64_t units = (slots * page_size + 63) / 64;
-  const PagedPlan plan = paged_plan(n_heads, n_kv_heads, seq_len, head_dim, dtype);
-  const int64_t blocks = plan.mfma ? batch * n_kv_heads * plan.tiles : batch * n_heads * seq_len;
-  // blocks of 4 waves a compute unit, of 4 units of 64 keys or more each
-  const int64_t want = (plan.mfma ? 2 : 8) * (int64_t)device_cu_count();
-  int64_t s = want / blocks;
+  const PagedPlan plan = paged_plan(batch, n_heads, n_kv_heads, seq_len, head_dim, dtype, 1);
+  if (plan.mfma) return paged_mfma_splits(plan, batch, n_kv_heads, head_dim, units, store);
+  const int64_t blocks = batch * n_heads * seq_len;
+  // 8 blocks of 4 waves a compute unit, of 4 units of 64 keys or more each
+  int64_t s = 8 * (int64_t)device_cu_count() / blocks;
   if (s > (units + 3) / 4) s = (units + 3) / 4;
-  return s < 1 ? 1 : (s > 256 ? 256 : s);
+  return ranges_per_row(s * batch, batch) * batch;
+}
+
+extern "C" int64_t mi_paged_attn_workspace(int64_t batch, int64_t n_heads, int64_t n_kv_heads,
+                                           int64_t seq_len, int64_t head_dim, int64_t num_splits,
+                                           int32_t dtype) {
+  if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || seq_len <= 0 || head_dim <= 0 ||
+      num_splits <= 1 || num_splits > MI_PAGED_ATTN_MAX_SPLITS || batch > (1 << 24) ||
+      n_heads > (1 << 16) || n_heads % n_kv_heads != 0 || seq_len > (1 << 24) || head_dim > 256)
+    return 0;
+  const PagedPlan plan =
+      paged_plan(batch, n_heads, n_kv_heads, seq_len, head_dim, dtype, num_splits);
+  if (plan.mfma) return paged_mfma_workspace(plan, n_kv_heads, head_dim);
+  const int64_t n = ranges_per_row(num_splits, batch);
+  return n > 1 ? batch * n_heads * seq_len * n * (head_dim + 2) : 0;
 }
 
 extern "C" int32_t mi_paged_attn(
@@ -287,8 +293,9 @@ extern "C" int32_t mi_paged_attn(
   if (int32_t st = paged_check("paged_attn", batch, n_heads, n_kv_heads, seq_len, head_dim,
                                num_pages, page_size, slots, dtype, store, scales))
     return st;
-  if (num_splits < 1 || num_splits > 256) {
-    set_last_error("paged_attn: num_splits must be 1..256, got %lld", (long long)num_splits);
+  if (num_splits < 1 || num_splits > MI_PAGED_ATTN_MAX_SPLITS) {
+    set_last_error("paged_attn: num_splits must be 1..%d, got %lld", MI_PAGED_ATTN_MAX_SPLITS,
+                   (long long)num_splits);
     return MI_ERR_INVALID;
   }
   if ((uintptr_t)k_pages % 16 != 0 || (uintptr_t)v_pages % 16 != 0) {
@@ -297,20 +304,30 @@ extern "C" int32_t mi_paged_attn(
   }
   if (batch == 0 || seq_len == 0) return MI_OK;
   const int64_t rows = batch * n_heads * seq_len;
-  if (rows > INT32_MAX) {
-    set_last_error("paged_attn: too many rows for one call");
+  const PagedPlan plan =
+      paged_plan(batch, n_heads, n_kv_heads, seq_len, head_dim, dtype, num_splits);
+  const int64_t ranges = plan.mfma ? 1 : ranges_per_row(num_splits, batch);
+  // (units of a list, blocks and rows are 32-bit)
+  if (rows > INT32_MAX || rows * ranges > INT32_MAX || plan.tiles > 65535 ||
+      n_kv_heads * (plan.parts > batch ? plan.parts : batch) > INT32_MAX ||
+      n_kv_heads * batch * plan.tiles > INT32_MAX ||
+      batch * ((slots * page_size + 63) / 64) > INT32_MAX ||
+      n_kv_heads * page_size * head_dim * 4 > UINT32_MAX) {
+    set_last_error("paged_attn: too many rows, keys and splits for one call");
     return MI_ERR_UNSUPPORTED;
   }
-  if (num_splits > 1 && (part == nullptr || part_elems < rows * num_splits * (head_dim + 2))) {
-    set_last_error("paged_attn: %lld splits need a workspace of %lld floats",
-                   (long long)num_splits, (long long)(rows * num_splits * (head_dim + 2)));
+  const int64_t need =
+      mi_paged_attn_workspace(batch, n_heads, n_kv_heads, seq_len, head_dim, num_splits, dtype);
+  if (need > 0 && (part == nullptr || (uintptr_t)part % 16 != 0 || part_elems < need)) {
+    set_last_error("paged_attn: %lld splits need a 16-byte aligned workspace of %lld floats",
+                   (long long)num_splits, (long long)need);
     return MI_ERR_INVALID;
   }
   PagedAttnArgs a{};
   a.q = q; a.kp = k_pages; a.vp = v_pages; a.scales = scales; a.table = page_table;
   a.seq_lens = seq_lens; a.lens = query_lens;
   a.part_acc = part;
-  a.part_ml = num_splits > 1 ? part + rows * num_splits * head_dim : nullptr;
+  a.part_ml = need > 0 ? part + need / (head_dim + 2) * head_dim : nullptr;
   a.out = out; a.lse = lse;
   a.q_sb = q_sb; a.q_sh = q_sh; a.q_ss = q_ss;
   a.o_sb = o_sb; a.o_sh = o_sh; a.o_ss = o_ss;
@@ -318,10 +335,10 @@ extern "C" int32_t mi_paged_attn(
   a.B = (int32_t)batch; a.Hq = (int32_t)n_heads; a.Hkv = (int32_t)n_kv_heads;
   a.group = (int32_t)(n_heads / n_kv_heads); a.S = (int32_t)seq_len; a.D = (int32_t)head_dim;
   a.P = (int32_t)page_size; a.p_shift = __builtin_ctzll((unsigned long long)page_size);
-  a.slots = (int32_t)slots; a.splits = (int32_t)num_splits;
+  a.slots = (int32_t)slots; a.splits = (int32_t)ranges;
+  a.tiles = (int32_t)plan.tiles; a.parts = (int32_t)plan.parts; a.kv_rows = 16 * plan.r;
   a.scale_log2 = sm_scale * kLog2e;
   const bool e8 = store == MI_STORE_E4M3;
-  const PagedPlan plan = paged_plan(n_heads, n_kv_heads, seq_len, head_dim, dtype);
   const int64_t es = dtype == MI_DTYPE_F32 ? 4 : 2;
   auto rows_of = [&](const void* p, int64_t n, std::initializer_list<int64_t> strides) {
     bool ok = (uintptr_t)p % n == 0;
@@ -331,13 +348,15 @@ extern "C" int32_t mi_paged_attn(
   a.q_vec = rows_of(q, 16, {q_sb, q_sh, q_ss});
   a.o_vec = rows_of(out, 8, {o_sb, o_sh, o_ss});
   hipStream_t st = (hipStream_t)stream;
-  int32_t rc;
-  if (dtype == MI_DTYPE_BF16)
-    rc = launch_attn<bf16_t>(a, plan, e8, st);
+  int32_t rc = MI_OK;
+  if (plan.mfma)
+    paged_attn_mfma_launch(a, plan, dtype, e8, st);
+  else if (dtype == MI_DTYPE_BF16)
+    rc = launch_attn<bf16_t>(a, e8, st);
   else if (dtype == MI_DTYPE_F16)
-    rc = launch_attn<f16_t>(a, plan, e8, st);
+    rc = launch_attn<f16_t>(a, e8, st);
   else
-    rc = launch_attn<float>(a, plan, e8, st);
+    rc = launch_attn<float>(a, e8, st);
   if (rc != MI_OK) return rc;
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

@@ -14,27 +14,32 @@ struct PagedAttnArgs {
   const int32_t* table;
   const int64_t* seq_lens;
   const int64_t* lens;      // query tokens of each row; null: S
-  float* part_acc;          // [B * Hq * S, splits, D]
-  float* part_ml;           // [B * Hq * S, splits, 2]
+  float* part_acc;          // sums of key ranges (unnormalised): one block a (row, range):
+  float* part_ml;           //   [B * Hq * S, splits, D] and [.., 2], their m and l
   void* out;
   float* lse;
   int64_t q_sb, q_sh, q_ss;
   int64_t o_sb, o_sh, o_ss;
   int64_t t_sb, num_pages;
   int32_t B, Hq, Hkv, group, S, D, P, p_shift, slots, splits;
+  int32_t tiles, parts, kv_rows;   // matrix cores: see PagedPlan; query rows of a block
   float scale_log2;
   int32_t q_vec, o_vec;     // q rows 16-byte, out rows 8-byte aligned
 };
 
-// How a call's rows are laid on blocks.
+// How a call is laid on blocks.
 struct PagedPlan {
-  bool mfma;       // the matrix-core kernel, else one block a (row, split)
-  int r;           // 16-row tiles of a wave
-  bool rows;       // a block's waves take different rows (else different keys)
-  int64_t tiles;   // blocks along the rows of a KV head
+  bool mfma;       // the matrix-core kernel, else one block a (query row, key range)
+  int r;           // 16-row tiles of a block
+  int64_t tiles;   // blocks along the query rows of a KV head
+  int64_t parts;   // blocks along a KV head's keys: parts of the list of all rows' keys,
+                   // or 0: one block a row (no second launch)
 };
-PagedPlan paged_plan(int64_t n_heads, int64_t n_kv_heads, int64_t seq_len, int64_t head_dim,
-                     int32_t dtype);
+PagedPlan paged_plan(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t seq_len,
+                     int64_t head_dim, int32_t dtype, int64_t num_splits);
+int64_t paged_mfma_splits(const PagedPlan& plan, int64_t batch, int64_t n_kv_heads,
+                          int64_t head_dim, int64_t units, int32_t store);
+int64_t paged_mfma_workspace(const PagedPlan& plan, int64_t n_kv_heads, int64_t head_dim);
 void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32_t dtype, bool e8,
                             hipStream_t st);
 

@@ -1,65 +1,64 @@
 // Launches of the matrix-core attention over a paged KV cache (paged_attn_mfma.hpp).
 #include "paged_attn_mfma.hpp"
 
-#ifndef V_ROWS_FROM
-#define V_ROWS_FROM 64
-#endif
-#ifndef V_PIPE1
-#define V_PIPE1 false
-#endif
-#ifndef V_PIPE2
-#define V_PIPE2 false
-#endif
-#ifndef V_RR
-#define V_RR 2
-#endif
-
 namespace mi {
 
-PagedPlan paged_plan(int64_t n_heads, int64_t n_kv_heads, int64_t seq_len, int64_t head_dim,
-                     int32_t dtype) {
+PagedPlan paged_plan(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t seq_len,
+                     int64_t head_dim, int32_t dtype, int64_t num_splits) {
   PagedPlan p{};
-  p.mfma = dtype != MI_DTYPE_F32 && head_dim % 64 == 0;
+  p.mfma = dtype != MI_DTYPE_F32 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
   if (!p.mfma) return p;
   const int64_t n = seq_len * (n_heads / n_kv_heads);
-  p.rows = n > V_ROWS_FROM;
   p.r = n <= 16 || head_dim > 128 ? 1 : 2;
-  if (p.rows && head_dim <= 128) p.r = V_RR;
-  const int64_t block = (p.rows ? 64 : 16) * p.r;
-  p.tiles = (n + block - 1) / block;
+  p.tiles = (n + 16 * p.r - 1) / (16 * p.r);
+  p.parts = num_splits <= 1 ? 0 : num_splits;
   return p;
+}
+
+int64_t paged_mfma_splits(const PagedPlan& plan, int64_t batch, int64_t n_kv_heads,
+                          int64_t head_dim, int64_t units, int32_t store) {
+  // blocks of 4 waves that are resident at once (by their registers)
+  const int64_t fill = (head_dim == 64 && plan.r == 1 ? 3 : head_dim == 256 ? 1 : 2) *
+                       (int64_t)device_cu_count();
+  const int64_t blocks = n_kv_heads * plan.tiles;
+  // a block a row where that is 4 rounds of blocks, or where no row has 8 units of keys
+  if (blocks * batch >= 4 * fill || units < 8) return 1;
+  int64_t parts = fill / blocks;
+  const int64_t most = batch * ((units + 3) / 4);
+  if (parts > most) parts = most;
+  return parts < 1 ? 1 : parts;
+}
+
+int64_t paged_mfma_workspace(const PagedPlan& plan, int64_t n_kv_heads, int64_t head_dim) {
+  return n_kv_heads * plan.tiles * plan.parts * 2 * (16 * plan.r) * (head_dim + 2);
 }
 
 namespace {
 
-template <typename T, bool E8, int D>
-void launch(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * a.splits), (unsigned)p.tiles), block(256);
-  if constexpr (D <= 128) {
-    if (p.rows)
-      hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, V_RR, true, false>), grid, block, 0, st, a);
-    else if (p.r == 2)
-      hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, 2, false, V_PIPE2>), grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, 1, false, V_PIPE1>), grid, block, 0, st, a);
-  } else {
-    if (p.rows)
-      hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, 1, true, false>), grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, 1, false, false>), grid, block, 0, st, a);
+template <typename T, bool E8, int D, int R>
+void launch_tiles(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(a.Hkv * (p.parts > 0 ? p.parts : a.B)), (unsigned)p.tiles);
+  if (p.tiles == 1)
+    hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, R, true>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_attn_mfma_kernel<T, E8, D, R, false>), grid, dim3(256), 0, st, a);
+  if (p.parts > 0) {
+    const int64_t blocks = (int64_t)a.B * a.Hkv * p.tiles;
+    // rows of a tile apart where their tiles alone are fewer than the compute units
+    const unsigned apart = blocks < device_cu_count() ? (unsigned)a.kv_rows : 1u;
+    hipLaunchKernelGGL((paged_mfma_join_kernel<T, D>), dim3((unsigned)blocks, apart), dim3(256), 0,
+                       st, a);
   }
 }
 
 template <typename T, bool E8>
-void launch_dim(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+void launch(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
   if (a.D == 64)
-    launch<T, E8, 64>(a, p, st);
+    p.r == 1 ? launch_tiles<T, E8, 64, 1>(a, p, st) : launch_tiles<T, E8, 64, 2>(a, p, st);
   else if (a.D == 128)
-    launch<T, E8, 128>(a, p, st);
-  else if (a.D == 192)
-    launch<T, E8, 192>(a, p, st);
+    p.r == 1 ? launch_tiles<T, E8, 128, 1>(a, p, st) : launch_tiles<T, E8, 128, 2>(a, p, st);
   else
-    launch<T, E8, 256>(a, p, st);
+    launch_tiles<T, E8, 256, 1>(a, p, st);
 }
 
 }  // namespace
@@ -67,9 +66,9 @@ void launch_dim(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
 void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32_t dtype, bool e8,
                             hipStream_t st) {
   if (dtype == MI_DTYPE_BF16)
-    e8 ? launch_dim<bf16_t, true>(a, plan, st) : launch_dim<bf16_t, false>(a, plan, st);
+    e8 ? launch<bf16_t, true>(a, plan, st) : launch<bf16_t, false>(a, plan, st);
   else
-    e8 ? launch_dim<f16_t, true>(a, plan, st) : launch_dim<f16_t, false>(a, plan, st);
+    e8 ? launch<f16_t, true>(a, plan, st) : launch<f16_t, false>(a, plan, st);
 }
 
 }  // namespace mi

@@ -23,11 +23,17 @@
 // (two products): off by 2^-16 at most, where one rounding of p to q's type would add an
 // error as large as that of the output itself.  l sums p in fp32.
 //
-// KEYS: the block's 4 waves take every 4th step of the block's key range and join
-// through LDS at the end (few rows: one token, a few drafts).  ROWS: the waves take
-// different row tiles over the same keys, which then come from the caches (a piece of
-// a prompt).  With PIPE two register sets alternate: the next step's 16 KB a wave are
-// on their way while this one is multiplied; page numbers are fetched a step earlier.
+// The block's 4 waves take every 4th step of its keys and join through LDS at the end.
+//
+// Blocks (parts > 0): the keys that the rows of the batch have, in units of 64, are one
+// list for each KV head and tile of query rows, and each block takes an equal part of
+// it: with lengths that differ 8-fold no block is longer than another.  A part that
+// starts or ends inside a row leaves the row's sums in the workspace, at most two such
+// per part, and paged_mfma_join_kernel adds them up.  parts = 0: a block takes a whole row.
+//
+// A load covers whole 128-byte lines where a key is one or more (a pair of loads takes
+// half-lines of its own rows and of rows 8 away, and the lanes exchange them), and is
+// non-temporal where no other block reads the same keys.
 //
 // Keys behind the last visible one: their scores are -inf and their V entries are
 // zeroed, so that nothing in them (a NaN in an old page) reaches a sum.  Where
@@ -52,6 +58,13 @@ template <> struct MatOp<bf16_t> {
   static __device__ inline uint32_t from_e4m3x2(uint32_t x, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, HI));
   }
+  // a and b rounded, and their rounded values
+  static __device__ inline uint32_t pack(float a, float b, float& ra, float& rb) {
+    const uint32_t w = __builtin_bit_cast(uint32_t, v2{(__bf16)a, (__bf16)b});
+    ra = __uint_as_float(w << 16);
+    rb = __uint_as_float(w & 0xffff0000u);
+    return w;
+  }
 };
 template <> struct MatOp<f16_t> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
@@ -62,6 +75,12 @@ template <> struct MatOp<f16_t> {
   template <bool HI>
   static __device__ inline uint32_t from_e4m3x2(uint32_t x, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, HI));
+  }
+  static __device__ inline uint32_t pack(float a, float b, float& ra, float& rb) {
+    const v2 w = {(_Float16)a, (_Float16)b};
+    ra = (float)w[0];
+    rb = (float)w[1];
+    return __builtin_bit_cast(uint32_t, w);
   }
 };
 
@@ -91,26 +110,40 @@ struct PagedGeom {
   static constexpr int STEP = 4 * CK;             // keys of a step
   static constexpr int KT = CK / 4;               // 16-key tiles of a step
   static constexpr int KL = E8 ? D / 64 : D / 32; // 16-byte loads of a key by a lane
+  static constexpr bool PAIRS = KL % 2 == 0;      // a key is whole 128-byte lines
   static constexpr int VL = D / 16;               // 16-byte loads of V by a lane
   static constexpr int U = CK / 8;                // P.V products' key groups of 32
   static constexpr int ES = E8 ? 1 : 2;
 };
 
-// One step's keys, as loaded.
+// One step's keys and values, as loaded.
 template <typename T, bool E8, int D>
-struct PagedStep {
+struct PagedK {
   typedef PagedGeom<T, E8, D> G;
   u32x4 k[G::KT][G::KL];
+  float scale;
+};
+template <typename T, bool E8, int D>
+struct PagedV {
+  typedef PagedGeom<T, E8, D> G;
   u32x4 v[G::VL];
-  float ks, vs;
-  int base;        // first key
-  bool live;       // the page of this lane's CK keys exists
+  float scale;
 };
 
-template <typename T, bool E8, int D, int R, bool ROWS, bool PIPE>
+#ifndef V_AHEAD
+#define V_AHEAD (!E8 && R == 1 && D == 128)
+#endif
+// Whether K of the next step is loaded ahead (where the registers hold it).
+template <bool E8, int D, int R>
+struct PagedAhead {
+  static constexpr bool value = V_AHEAD;
+};
+
+template <typename T, bool E8, int D, int R, bool STREAM>
 struct PagedWave {
   typedef PagedGeom<T, E8, D> G;
-  typedef PagedStep<T, E8, D> Step;
+  typedef PagedK<T, E8, D> KStep;
+  typedef PagedV<T, E8, D> VStep;
   typedef typename std::conditional<E8, bf16_t, T>::type PT;   // what P and V multiply in
   typedef typename MatOp<T>::v8 Q8;
   typedef typename MatOp<PT>::v8 P8;
@@ -119,8 +152,8 @@ struct PagedWave {
   const unsigned char* vp;
   const float* scales;
   const int32_t* table;
-  int64_t page_stride;        // bytes of a page (all heads)
-  int64_t num_pages;
+  uint32_t page_stride;       // bytes of a page (all heads; the host checks that they fit)
+  uint32_t num_pages;
   int Hkv, P, p_shift, slots;
   int lane, g, r;
   int lo, lim, minvis;        // keys [lo, lim); all rows that see any of them see [lo, minvis)
@@ -135,39 +168,101 @@ struct PagedWave {
     const int s = key >> p_shift;
     return table[s < slots ? s : slots - 1];
   }
-  __device__ inline void lookup(int base, int32_t* pk, int32_t* pv) const {
-    *pk = page_of(base + ((r >> 2) * G::CK));
-    *pv = page_of(base + g * G::CK);
-  }
-  __device__ inline void load(Step& st, int base, int32_t pk, int32_t pv) const {
-    // K: this lane's key of tile t is chunk r / 4, key 4t + r % 4; V: chunk g, dim r
-    const int kc = base + (r >> 2) * G::CK, vc = base + g * G::CK;
-    const bool kok = kc < lim && pk >= 0 && pk < num_pages;
-    const bool vok = vc < lim && pv >= 0 && pv < num_pages;
-    // (page 0 stands in where there is none: what it gives is masked)
-    const unsigned char* ka = kp + (kok ? (int64_t)pk : 0) * page_stride +
-                              (((kc & (P - 1)) + (r & 3)) * D + g * (16 / G::ES)) * G::ES;
-    const unsigned char* va = vp + (vok ? (int64_t)pv : 0) * page_stride +
-                              (r * P + (vc & (P - 1))) * G::ES;
-#pragma unroll
-    for (int t = 0; t < G::KT; ++t)
-#pragma unroll
-      for (int i = 0; i < G::KL; ++i) st.k[t][i] = load16(ka + t * 4 * D * G::ES + i * 64);
-    const int vrow = 16 * P * G::ES;
-#pragma unroll
-    for (int i = 0; i < G::VL; ++i) st.v[i] = load16(va + i * vrow);
-    st.ks = st.vs = 1.0f;
-    if constexpr (E8) {
-      if (vok) {
-        const float* sc = scales + (int64_t)pv * Hkv * 2;
-        st.ks = sc[0];
-        st.vs = sc[1];
-      }
+  // pages of the step's keys that this lane loads
+  struct Pages {
+    int32_t k0, k1, v;
+  };
+  __device__ inline Pages lookup(int base) const {
+    Pages p;
+    if constexpr (G::PAIRS) {
+      p.k0 = page_of(base + ((r & 7) >> 2) * G::CK);
+      p.k1 = page_of(base + (2 + ((r & 7) >> 2)) * G::CK);
+    } else {
+      p.k0 = p.k1 = page_of(base + (r >> 2) * G::CK);
     }
-    st.base = base;
-    st.live = vok;
+    p.v = page_of(base + g * G::CK);
+    return p;
+  }
+  // where a page's chunk of CK keys lies; page 0 stands in where there is none (what it
+  // gives is masked)
+  __device__ inline bool chunk(int key, int32_t page, int64_t* at) const {
+    const bool ok = key < lim && (uint32_t)page < num_pages;
+    *at = (int64_t)((uint64_t)(ok ? (uint32_t)page : 0u) * page_stride);
+    return ok;
+  }
+  __device__ inline u32x4 fetch(const unsigned char* p) const {
+    return STREAM ? load16_stream(p) : load16(p);
+  }
+  __device__ inline float page_scale(int32_t page, bool ok, int which) const {
+    if constexpr (E8) {
+      if (ok) return scales[(uint64_t)(uint32_t)page * (uint32_t)(2 * Hkv) + which];
+    }
+    return 1.0f;
+  }
+  __device__ inline void load_k(KStep& st, int base, const Pages& pg) const {
+    int64_t at;
+    if constexpr (G::PAIRS) {
+      // Two loads of a pair take rows 0..7 and 8..15 of the tile, lanes r < 8 the first and
+      // r >= 8 the second 64 bytes of a 128-byte line: each load takes whole lines
+      // (fold exchanges them).
+      const int key0 = base + ((r & 7) >> 2) * G::CK, key1 = key0 + 2 * G::CK;
+      const int in_line = (r >> 3) * 64 + g * 16;
+      chunk(key0, pg.k0, &at);
+      const unsigned char* k0 = kp + at + ((key0 & (P - 1)) + (r & 3)) * D * G::ES + in_line;
+      chunk(key1, pg.k1, &at);
+      const unsigned char* k1 = kp + at + ((key1 & (P - 1)) + (r & 3)) * D * G::ES + in_line;
+#pragma unroll
+      for (int t = 0; t < G::KT; ++t)
+#pragma unroll
+        for (int i = 0; i < G::KL; i += 2) {
+          st.k[t][i] = fetch(k0 + t * 4 * D * G::ES + i * 64);
+          st.k[t][i + 1] = fetch(k1 + t * 4 * D * G::ES + i * 64);
+        }
+    } else {
+      const int key = base + (r >> 2) * G::CK;
+      chunk(key, pg.k0, &at);
+      const unsigned char* k0 = kp + at + ((key & (P - 1)) + (r & 3)) * D * G::ES + g * 16;
+#pragma unroll
+      for (int t = 0; t < G::KT; ++t) st.k[t][0] = fetch(k0 + t * 4 * D * G::ES);
+    }
+    st.scale = page_scale(pg.v, live(base, pg), 0);   // of the keys whose scores this lane gets
+  }
+  // the page of this lane's CK keys exists
+  __device__ inline bool live(int base, const Pages& pg) const {
+    return base + g * G::CK < lim && (uint32_t)pg.v < num_pages;
+  }
+  __device__ inline void load_v(VStep& st, int base, const Pages& pg) const {
+    int64_t at;
+    const int key = base + g * G::CK;
+    const bool ok = chunk(key, pg.v, &at);
+    const unsigned char* va = vp + at + (r * P + (key & (P - 1))) * G::ES;
+#pragma unroll
+    for (int i = 0; i < G::VL; ++i) st.v[i] = fetch(va + i * 16 * P * G::ES);
+    st.scale = page_scale(pg.v, ok, 1);
+  }
+  // x for lanes of `banks` (0xc: r >= 8, 0x3: r < 8) from lane r ^ 8 of y
+  template <int BANKS>
+  static __device__ inline uint32_t from_other_half(uint32_t x, uint32_t y) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)y, 0x128, 0xf, BANKS, false);
+  }
+  // the 64-byte pieces of row r, from a pair of loads
+  __device__ inline void exchange(u32x4& a, u32x4& b) const {
+    const u32x4 x = a, y = b;
+    a = u32x4{from_other_half<0xc>(x.x, y.x), from_other_half<0xc>(x.y, y.y),
+              from_other_half<0xc>(x.z, y.z), from_other_half<0xc>(x.w, y.w)};
+    b = u32x4{from_other_half<0x3>(y.x, x.x), from_other_half<0x3>(y.y, x.y),
+              from_other_half<0x3>(y.z, x.z), from_other_half<0x3>(y.w, x.w)};
   }
 
+  // K operand j (32 dims) of tile t
+  __device__ inline Q8 k_op(const KStep& st, int t, int j) const {
+    if constexpr (E8) {
+      const u32x4 w = st.k[t][j >> 1];
+      return (j & 1) ? widen8<T>(w.z, w.w, 1.0f) : widen8<T>(w.x, w.y, 1.0f);
+    } else {
+      return __builtin_bit_cast(Q8, st.k[t][j]);
+    }
+  }
   // V operand u of dims 16 i .. 16 i + 15
   __device__ inline P8 v_op(const u32x4& v, int u, float vs) const {
     if constexpr (E8)
@@ -204,41 +299,56 @@ struct PagedWave {
     return w & ~((not_finite(w) >> (8 * G::ES - 1)) * (E8 ? 0xffu : 0xffffu));
   }
 
-  __device__ inline void fold(Step& st) {
-    const int cb = st.base + g * G::CK;
+  P8 hi[R][G::U], rest[R][G::U];   // p of the step: its 16-bit value and the remainder
+  bool whole, here;                // the step's keys are all seen by all rows; `live`
+
+  // scores, softmax and p of the step at `base`
+  __device__ inline void fold_k(KStep& st, int base, const Pages& pg) {
+    const int cb = base + g * G::CK;
+    here = live(base, pg);
     f32x4 s[R][G::KT];
+    // two tiles at a time: products into one accumulator wait for each other
 #pragma unroll
-    for (int t = 0; t < G::KT; ++t) {
+    for (int t = 0; t < G::KT; t += 2) {
+      if constexpr (G::PAIRS) {
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) s[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < G::KL; i += 2) {
+          exchange(st.k[t][i], st.k[t][i + 1]);
+          exchange(st.k[t + 1][i], st.k[t + 1][i + 1]);
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) s[rt][t] = s[rt][t + 1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
-        Q8 a;
-        if constexpr (E8) {
-          const u32x4 w = st.k[t][j >> 1];
-          a = (j & 1) ? widen8<T>(w.z, w.w, 1.0f) : widen8<T>(w.x, w.y, 1.0f);
-        } else {
-          a = __builtin_bit_cast(Q8, st.k[t][j]);
-        }
+        const Q8 a0 = k_op(st, t, j), a1 = k_op(st, t + 1, j);
 #pragma unroll
-        for (int rt = 0; rt < R; ++rt) s[rt][t] = MatOp<T>::mul(a, q[rt][j], s[rt][t]);
+        for (int rt = 0; rt < R; ++rt) {
+          s[rt][t] = MatOp<T>::mul(a0, q[rt][j], s[rt][t]);
+          s[rt][t + 1] = MatOp<T>::mul(a1, q[rt][j], s[rt][t + 1]);
+        }
       }
     }
-    const float c = E8 ? st.ks * scale_log2 : scale_log2;
+    const float c = E8 ? st.scale * scale_log2 : scale_log2;
     // every row sees all keys of the step, and their pages exist
-    const bool whole = st.base + G::STEP <= minvis && __all(st.live);
-    P8 hi[R][G::U], rest[R][G::U];
+    whole = base + G::STEP <= minvis && __all(here);
+    if (!whole) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        const int n = here ? vis[rt] - cb : 0;     // keys of this lane's that the row sees
+#pragma unroll
+        for (int e = 0; e < G::CK; ++e)
+          s[rt][e >> 2][e & 3] = e < n ? s[rt][e >> 2][e & 3] : -INFINITY;
+      }
+      asm volatile("");   // (a branch: selects would cost every step)
+    }
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
-      const int n = whole ? G::CK : (st.live ? vis[rt] - cb : 0);   // keys of this lane's that the row sees
-      float x[G::CK];
-      float top = kNegBig;
+      // the largest of the unscaled scores (the scale is positive and one for the lane's keys)
+      float top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < G::CK; ++e) {
-        x[e] = s[rt][e >> 2][e & 3] * c;
-        if (!whole) x[e] = e < n ? x[e] : -INFINITY;
-        top = fmaxf(top, x[e]);
-      }
+      for (int e = 0; e < G::CK; ++e) top = fmaxf(top, s[rt][e >> 2][e & 3]);
+      top *= c;
       top = fmaxf(top, swap16(top, lane));
       top = fmaxf(top, swap32(top, lane));
       const float m_new = fmaxf(m[rt], top);
@@ -251,20 +361,29 @@ struct PagedWave {
       float sum = 0.0f;
 #pragma unroll
       for (int u = 0; u < G::U; ++u) {
+        uint32_t h[4], x[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = fast_exp2(x[8 * u + e] - m_new);
-          sum += p;
-          const PT h = (PT)p;
-          hi[rt][u][e] = h;
-          rest[rt][u][e] = (PT)(p - (float)h);
+        for (int e = 0; e < 4; ++e) {
+          const int k = 8 * u + 2 * e;
+          const float p0 = fast_exp2(fmaf(s[rt][k >> 2][k & 3], c, -m_new));
+          const float p1 = fast_exp2(fmaf(s[rt][k >> 2][(k & 3) + 1], c, -m_new));
+          sum += p0 + p1;
+          float h0, h1;
+          h[e] = MatOp<PT>::pack(p0, p1, h0, h1);
+          x[e] = MatOp<PT>::pack(p0 - h0, p1 - h1, h0, h1);
         }
+        hi[rt][u] = __builtin_bit_cast(P8, u32x4{h[0], h[1], h[2], h[3]});
+        rest[rt][u] = __builtin_bit_cast(P8, u32x4{x[0], x[1], x[2], x[3]});
       }
       l[rt] = l[rt] * alpha + sum;
     }
+  }
+
+  // o += V^T P^T
+  __device__ inline void fold_v(VStep& st, int base) {
     bool odd = false;
     if (!whole) {
-      const int n = st.live ? lim - cb : 0;
+      const int n = here ? lim - (base + g * G::CK) : 0;
 #pragma unroll
       for (int i = 0; i < G::VL; ++i) st.v[i] = keep(st.v[i], 0, n);
       if (minvis < lim) {
@@ -283,19 +402,27 @@ struct PagedWave {
         }
       }
     }
+    constexpr int kTogether = 2;   // dims' accumulators in turn, as above
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
+    for (int i = 0; i < D / 16; i += kTogether) {
 #pragma unroll
       for (int u = 0; u < G::U; ++u) {
-        const P8 a = v_op(st.v[i], u, st.vs);
+        P8 a[kTogether];
+#pragma unroll
+        for (int j = 0; j < kTogether; ++j) a[j] = v_op(st.v[i + j], u, st.scale);
 #pragma unroll
         for (int rt = 0; rt < R; ++rt) {
-          o[rt][i] = MatOp<PT>::mul(a, hi[rt][u], o[rt][i]);
-          o[rt][i] = MatOp<PT>::mul(a, rest[rt][u], o[rt][i]);
+#pragma unroll
+          for (int j = 0; j < kTogether; ++j) o[rt][i + j] = MatOp<PT>::mul(a[j], hi[rt][u], o[rt][i + j]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) {
+#pragma unroll
+          for (int j = 0; j < kTogether; ++j) o[rt][i + j] = MatOp<PT>::mul(a[j], rest[rt][u], o[rt][i + j]);
         }
       }
     }
-    if (odd) add_not_finite(st.base);
+    if (odd) add_not_finite(base);
   }
 
   // The entries of a step that are not finite, added to the rows that see their keys (the
@@ -306,8 +433,8 @@ struct PagedWave {
 #pragma unroll 1
     for (int key = base; key < end; ++key) {
       const int32_t page = page_of(key);
-      if (page < 0 || page >= num_pages) continue;
-      const unsigned char* p = vp + page * page_stride + (4 * g * P + (key & (P - 1))) * G::ES;
+      if ((uint32_t)page >= num_pages) continue;
+      const unsigned char* p = vp + (int64_t)((uint64_t)page * page_stride) + (4 * g * P + (key & (P - 1))) * G::ES;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
@@ -328,23 +455,112 @@ struct PagedWave {
   }
 };
 
-template <typename T, bool E8, int D, int R, bool ROWS, bool PIPE>
-__global__ __launch_bounds__(256, D > 128 || (PIPE && R > 1) ? 1 : 2) void paged_attn_mfma_kernel(PagedAttnArgs a) {
-  typedef PagedWave<T, E8, D, R, ROWS, PIPE> Wave;
+// ------------------------------------------------ the list of a KV head's keys
+// Rows b = 0 .. B-1, each with ceil(vis / 64) units, vis the keys that the last query
+// row of a tile sees.  A wave holds 64 rows of it at a time, one a lane.
+struct UnitList {
+  const PagedAttnArgs* a;
+  int s_first, s_last;       // query tokens of the tile's first and last row
+  int lane;
+  int b0;                    // first row held
+  int units, end;            // the lane's row: its units, and the list's up to it
+  int before;                // units of the rows before b0
+
+  __device__ inline int vis_of(const RowKeys& rk) const {
+    // the last query token that is real (tokens behind query_lens see nothing)
+    return s_first < rk.n ? rk.vis(s_last < rk.n ? s_last : rk.n - 1) : 0;
+  }
+  __device__ inline void hold(int first, int units_before) {
+    b0 = first;
+    before = units_before;
+    const int b = first + lane;
+    units = b < a->B ? (vis_of(row_keys(*a, b)) + 63) >> 6 : 0;
+    end = units;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+      const int x = __shfl_up(end, i, 64);
+      if (lane >= i) end += x;
+    }
+    end += before;
+  }
+  __device__ inline int held_end() const { return __builtin_amdgcn_readlane(end, 63); }
+  // the whole list's units; rows [0, 64) are held afterwards
+  __device__ inline int total() {
+    int t = 0;
+    for (int b = (a->B - 1) / 64 * 64; b > 0; b -= 64) {
+      hold(b, 0);
+      t += held_end();
+    }
+    hold(0, 0);
+    return t + held_end();
+  }
+};
+// parts in use (4 units each at least), and where part i of a list of `total` units starts
+__device__ inline int parts_used(int total, int parts) {
+  const int most = (total + 3) >> 2;
+  return most < parts ? most : parts;
+}
+__device__ inline int part_start(int i, int total, int used) {
+  return (int)((int64_t)i * total / used);
+}
+// workspace: sums (D floats) and m, l of the two ends of each part
+__device__ inline int64_t part_at(const PagedAttnArgs& a, int hk, int tile, int part, int end) {
+  return ((((int64_t)hk * a.tiles + tile) * a.parts + part) * 2 + end) * a.kv_rows;
+}
+
+template <typename T>
+__device__ inline void store_row4(const PagedAttnArgs& a, int b, int h, int s, int d, f32x4 v,
+                                  float M, float L) {
+  T* op = static_cast<T*>(a.out) + b * a.o_sb + h * a.o_sh + s * a.o_ss + d;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? (T)0.0f : Elem<T>::from_f32(v[e] / L);
+  if (a.o_vec) {
+    *reinterpret_cast<t4*>(op) = y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) op[e] = y[e];
+  }
+  if (d == 0 && a.lse != nullptr)
+    a.lse[((int64_t)b * a.Hq + h) * a.S + s] = L == 0.0f ? -INFINITY : (M + fast_log2(L)) * kLn2;
+}
+
+template <typename T, bool E8, int D, int R, bool STREAM>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(PagedAttnArgs a) {
+  typedef PagedWave<T, E8, D, R, STREAM> Wave;
   typedef PagedGeom<T, E8, D> G;
-  typedef PagedStep<T, E8, D> Step;
+  constexpr int kRows = 16 * R;
   constexpr int kPitch = D + 4;                    // of a row in LDS: rows fall on different banks
-  __shared__ float acc_s[ROWS ? 1 : 4 * 16 * R * kPitch];
-  __shared__ float ml_s[ROWS ? 1 : 4 * 16 * R * 2];
+  __shared__ float acc_s[4 * kRows * kPitch];
+  __shared__ float ml_s[4 * kRows * 2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int blk = blockIdx.x;
-  const int split = blk % a.splits; blk /= a.splits;
-  const int hk = blk % a.Hkv, b = blk / a.Hkv;
-  const int n_rows = a.S * a.group;                // rows of this KV head
-  const int block_row = blockIdx.y * (ROWS ? 64 * R : 16 * R);
-  const int row0 = ROWS ? block_row + wave * 16 * R : block_row;
-  const RowKeys rk = row_keys(a, b);
+  const int hk = blockIdx.x % a.Hkv, part = blockIdx.x / a.Hkv, tile = blockIdx.y;
+  const int n_rows = a.S * a.group;                // query rows of this KV head
+  const int row0 = tile * kRows;
+  const int last = (row0 + kRows < n_rows ? row0 + kRows : n_rows) - 1;
+
+  UnitList list;
+  list.a = &a;
+  list.lane = lane;
+  list.s_first = row0 / a.group;
+  list.s_last = last / a.group;
+
+  // this block's units [u, u1) and the row b that they start in, whose units start at row_u
+  int b = part, u = 0, u1 = 0, row_u = 0;
+  if (a.parts > 0) {
+    const int total = list.total();
+    const int used = parts_used(total, a.parts);
+    if (part >= used) return;
+    u = part_start(part, total, used);
+    u1 = part_start(part + 1, total, used);
+    while (list.held_end() <= u) list.hold(list.b0 + 64, list.held_end());
+    const int at = (int)__builtin_ctzll(__ballot(list.end > u));
+    b = list.b0 + at;
+    row_u = __builtin_amdgcn_readlane(list.end, at) - __builtin_amdgcn_readlane(list.units, at);
+  }
+  const int u0 = u;
 
   Wave w;
   w.lane = lane;
@@ -353,145 +569,112 @@ __global__ __launch_bounds__(256, D > 128 || (PIPE && R > 1) ? 1 : 2) void paged
   const int64_t head_bytes = (int64_t)a.P * D * G::ES;
   w.kp = static_cast<const unsigned char*>(a.kp) + hk * head_bytes;
   w.vp = static_cast<const unsigned char*>(a.vp) + hk * head_bytes;
-  w.page_stride = head_bytes * a.Hkv;
+  w.page_stride = (uint32_t)(head_bytes * a.Hkv);
   w.scales = E8 ? a.scales + 2 * hk : nullptr;
-  w.table = a.table + (int64_t)b * a.t_sb;
-  w.num_pages = a.num_pages;
+  w.num_pages = (uint32_t)a.num_pages;
   w.Hkv = a.Hkv; w.P = a.P; w.p_shift = a.p_shift; w.slots = a.slots;
   w.scale_log2 = a.scale_log2;
 
-  // keys of the block: those its last row sees, this split's part of them
-  auto last_vis = [&](int first, int count) {      // of rows [first, first + count)
-    const int last = first + count < n_rows ? first + count : n_rows;
-    if (first >= last) return 0;
-    const int s_hi = (last - 1) / a.group;
-    return rk.vis(s_hi < rk.n ? s_hi : (rk.n > 0 && first / a.group < rk.n ? rk.n - 1 : s_hi));
-  };
-  int hi;
-  split_range(last_vis(block_row, ROWS ? 64 * R : 16 * R), split, a.splits, &w.lo, &hi);
-  if (ROWS) {
-    const int own = last_vis(row0, 16 * R);
-    hi = own < hi ? own : hi;
-  }
-  w.lim = hi;
-  w.minvis = row0 < n_rows ? rk.vis(row0 / a.group) : 0;
-  w.minvis = w.minvis > w.lo ? w.minvis : w.lo;
-
-#pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    const int row = row0 + 16 * rt + w.r;
-    const int s = row / a.group, hg = row - s * a.group;
-    const bool real = row < n_rows;
-    w.vis[rt] = real ? rk.vis(s) : 0;
-    w.m[rt] = kNegBig;
-    w.l[rt] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) w.o[rt][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + (hk * a.group + hg) * a.q_sh + s * a.q_ss;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      // the dims of K's operand j
-      const int d = E8 ? (j >> 1) * 64 + w.g * 16 + (j & 1) * 8 : j * 32 + w.g * 8;
-      typename Wave::Q8 x;
-      if (!real) {
-        x = __builtin_bit_cast(typename Wave::Q8, u32x4{0u, 0u, 0u, 0u});
-      } else if (a.q_vec) {
-        x = __builtin_bit_cast(typename Wave::Q8, load16(qp + d));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = qp[d + e];
-      }
-      w.q[rt][j] = x;
+  for (;;) {
+    const RowKeys rk = row_keys(a, b);
+    const int vis = list.vis_of(rk);
+    const int units = (vis + 63) >> 6;
+    int hi = vis;
+    bool whole = true;       // this block has all of the row's keys
+    w.lo = 0;
+    if (a.parts > 0) {
+      const int from = u - row_u, to = u1 - row_u < units ? u1 - row_u : units;
+      whole = from == 0 && to == units;
+      w.lo = from * 64;
+      hi = to * 64 < vis ? to * 64 : vis;
     }
-  }
-
-  const int stride = ROWS ? G::STEP : 4 * G::STEP;
-  int base = w.lo + (ROWS ? 0 : wave * G::STEP);
-  if (base < hi) {
-    int32_t pk, pv;
-    if constexpr (PIPE) {
-      Step x, y;
-      w.lookup(base, &pk, &pv);
-      w.load(x, base, pk, pv);
-      w.lookup(base + stride, &pk, &pv);
-      for (;;) {
-        base += stride;
-        const bool more = base < hi;
-        if (more) {
-          w.load(y, base, pk, pv);
-          w.lookup(base + stride, &pk, &pv);
-        }
-        w.fold(x);
-        if (!more) break;
-        base += stride;
-        const bool again = base < hi;
-        if (again) {
-          w.load(x, base, pk, pv);
-          w.lookup(base + stride, &pk, &pv);
-        }
-        w.fold(y);
-        if (!again) break;
-      }
-    } else {
-      Step x;
-      w.lookup(base, &pk, &pv);
-      for (; base < hi; base += stride) {
-        w.load(x, base, pk, pv);
-        w.lookup(base + stride, &pk, &pv);
-        w.fold(x);
-      }
-    }
-  }
-#pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    w.l[rt] += swap16(w.l[rt], lane);
-    w.l[rt] += swap32(w.l[rt], lane);
-    if (w.vis[rt] == 0) {   // no query token (whole steps do not look at each row's keys)
-      w.m[rt] = kNegBig;
-      w.l[rt] = 0.0f;
-    }
-  }
-
-  // where 4 dims from d of a row go
-  auto put = [&](int row, int d, f32x4 v, float M, float L) {
-    const int s = row / a.group, h = hk * a.group + row - s * a.group;
-    if (a.splits > 1) {
-      const int64_t at = (((int64_t)b * a.Hq + h) * a.S + s) * a.splits + split;
-      *reinterpret_cast<f32x4*>(a.part_acc + at * D + d) = v;
-      if (d == 0) {
-        a.part_ml[2 * at] = M;
-        a.part_ml[2 * at + 1] = L;
-      }
-      return;
-    }
-    T* op = static_cast<T*>(a.out) + b * a.o_sb + h * a.o_sh + s * a.o_ss + d;
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    t4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = L == 0.0f ? (T)0.0f : Elem<T>::from_f32(v[e] / L);
-    if (a.o_vec) {
-      *reinterpret_cast<t4*>(op) = y;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) op[e] = y[e];
-    }
-    if (d == 0 && a.lse != nullptr)
-      a.lse[((int64_t)b * a.Hq + h) * a.S + s] = L == 0.0f ? -INFINITY : (M + fast_log2(L)) * kLn2;
-  };
-
-  if constexpr (ROWS) {
+    w.lim = hi;
+    w.minvis = rk.vis(list.s_first);
+    w.minvis = w.minvis > w.lo ? w.minvis : w.lo;
+    w.table = a.table + (int64_t)b * a.t_sb;
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
       const int row = row0 + 16 * rt + w.r;
-      if (row < n_rows) {
+      const int s = row / a.group, hg = row - s * a.group;
+      const bool real = row < n_rows;
+      w.vis[rt] = real ? rk.vis(s) : 0;
+      w.m[rt] = kNegBig;
+      w.l[rt] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) put(row, 16 * i + 4 * w.g, w.o[rt][i], w.m[rt], w.l[rt]);
+      for (int i = 0; i < D / 16; ++i) w.o[rt][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const T* qp =
+          static_cast<const T*>(a.q) + b * a.q_sb + (hk * a.group + hg) * a.q_sh + s * a.q_ss;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        // the dims of K's operand j
+        const int d = E8 ? (j >> 1) * 64 + w.g * 16 + (j & 1) * 8 : j * 32 + w.g * 8;
+        typename Wave::Q8 x;
+        if (!real) {
+          x = __builtin_bit_cast(typename Wave::Q8, u32x4{0u, 0u, 0u, 0u});
+        } else if (a.q_vec) {
+          x = __builtin_bit_cast(typename Wave::Q8, load16(qp + d));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = qp[d + e];
+        }
+        w.q[rt][j] = x;
       }
     }
-  } else {
+
+    int base = w.lo + wave * G::STEP;
+    if (base < hi) {
+      constexpr int kStride = 4 * G::STEP;
+      typename Wave::Pages pg = w.lookup(base), next = w.lookup(base + kStride);
+      typename Wave::VStep v;
+      if constexpr (PagedAhead<E8, D, R>::value) {
+        // K of the next step is on its way from before this step's products, V of the next
+        // from behind them
+        typename Wave::KStep ka, kb;
+        w.load_k(ka, base, pg);
+        w.load_v(v, base, pg);
+        for (;;) {
+          const bool more = base + kStride < hi;
+          if (more) w.load_k(kb, base + kStride, next);
+          w.fold_k(ka, base, pg);
+          w.fold_v(v, base);
+          if (!more) break;
+          base += kStride;
+          w.load_v(v, base, next);
+          pg = next;
+          next = w.lookup(base + kStride);
+          const bool again = base + kStride < hi;
+          if (again) w.load_k(ka, base + kStride, next);
+          w.fold_k(kb, base, pg);
+          w.fold_v(v, base);
+          if (!again) break;
+          base += kStride;
+          w.load_v(v, base, next);
+          pg = next;
+          next = w.lookup(base + kStride);
+        }
+      } else {
+        typename Wave::KStep k;
+        for (; base < hi; base += kStride) {
+          w.load_k(k, base, pg);
+          w.load_v(v, base, pg);
+          w.fold_k(k, base, pg);
+          w.fold_v(v, base);
+          pg = next;
+          next = w.lookup(base + 2 * kStride);
+        }
+      }
+    }
+
+    // the block's waves, joined
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
-      const int at = wave * 16 * R + 16 * rt + w.r;
+      w.l[rt] += swap16(w.l[rt], lane);
+      w.l[rt] += swap32(w.l[rt], lane);
+      if (w.vis[rt] == 0) {   // no query token (whole steps do not look at each row's keys)
+        w.m[rt] = kNegBig;
+        w.l[rt] = 0.0f;
+      }
+      const int at = wave * kRows + 16 * rt + w.r;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
         *reinterpret_cast<f32x4*>(acc_s + at * kPitch + 16 * i + 4 * w.g) = w.o[rt][i];
@@ -501,23 +684,117 @@ __global__ __launch_bounds__(256, D > 128 || (PIPE && R > 1) ? 1 : 2) void paged
       }
     }
     __syncthreads();
-    for (int it = tid; it < 16 * R * (D / 4); it += 256) {
+    const int64_t slot = whole ? 0 : part_at(a, hk, tile, part, u == u0 ? 0 : 1);
+    for (int it = tid; it < kRows * (D / 4); it += 256) {
       const int rr = it / (D / 4), d = 4 * (it % (D / 4));
-      if (block_row + rr >= n_rows) continue;
+      if (row0 + rr >= n_rows) continue;
       float M = kNegBig, L = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) M = fmaxf(M, ml_s[2 * (i * 16 * R + rr)]);
+      for (int i = 0; i < 4; ++i) M = fmaxf(M, ml_s[2 * (i * kRows + rr)]);
       f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = i * 16 * R + rr;
+        const int at = i * kRows + rr;
         const float li = ml_s[2 * at + 1];
         if (li == 0.0f) continue;                  // the wave's keys are none of this row's
         const float f = fast_exp2(ml_s[2 * at] - M);
         L += f * li;
         v += f * *reinterpret_cast<const f32x4*>(acc_s + at * kPitch + d);
       }
-      put(block_row + rr, d, v, M, L);
+      if (whole) {
+        const int row = row0 + rr, s = row / a.group;
+        store_row4<T>(a, b, hk * a.group + row - s * a.group, s, d, v, M, L);
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_acc + (slot + rr) * D + d) = v;
+        if (d == 0) {
+          a.part_ml[2 * (slot + rr)] = M;
+          a.part_ml[2 * (slot + rr) + 1] = L;
+        }
+      }
+    }
+    // the next row with keys
+    if (a.parts == 0) break;
+    u = row_u + units;
+    if (u >= u1) break;
+    __syncthreads();                               // LDS is written again
+    while (list.held_end() <= u) list.hold(list.b0 + 64, list.held_end());
+    const int at = (int)__builtin_ctzll(__ballot(list.end > u));
+    b = list.b0 + at;
+    row_u = u;
+  }
+}
+
+// Rows whose keys several parts had: sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
+// over them.  Rows without keys become 0; all others are written already.  A block takes
+// the query rows of one tile (or, where that leaves most of the GPU idle, one of
+// them), D / 4 threads a part's sums (4 dims each): with up to 4 parts the groups take
+// a query row each, else they share the parts of one.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
+  constexpr int kGroups = 256 / (D / 4);
+  __shared__ f32x4 acc_s[256];
+  __shared__ float l_s[kGroups];
+  const int tid = threadIdx.x, lane = tid & 63;
+  int blk = blockIdx.x;
+  const int hk = blk % a.Hkv; blk /= a.Hkv;
+  const int tile = blk % a.tiles, b = blk / a.tiles;
+  const int n_rows = a.S * a.group, row0 = tile * a.kv_rows;
+  const int rows = row0 + a.kv_rows < n_rows ? a.kv_rows : n_rows - row0;
+  UnitList list;
+  list.a = &a;
+  list.lane = lane;
+  list.s_first = row0 / a.group;
+  list.s_last = (row0 + rows - 1) / a.group;
+  const int total = list.total();
+  while (list.b0 + 64 <= b) list.hold(list.b0 + 64, list.held_end());
+  const int end = __builtin_amdgcn_readlane(list.end, b - list.b0);
+  const int units = __builtin_amdgcn_readlane(list.units, b - list.b0);
+  const int first_u = end - units;
+  const int grp = tid / (D / 4), d = 4 * (tid % (D / 4));
+  // the part that holds unit x is the last one that starts at x or before
+  const int used = parts_used(total, a.parts);
+  int i0 = 0, i1 = -1, end0 = 0;
+  if (units > 0) {
+    i0 = (int)((((int64_t)first_u + 1) * used - 1) / total);
+    i1 = (int)(((int64_t)end * used - 1) / total);
+    if (i0 == i1) return;
+    // (in part i0 the row is the last one, unless it starts with it; in the others the first)
+    end0 = part_start(i0, total, used) == first_u ? 0 : 1;
+  }
+  const bool share = i1 - i0 >= 4;
+  for (int rr = blockIdx.y + (share ? 0 : (int)gridDim.y * grp); rr < rows;
+       rr += (int)gridDim.y * (share ? 1 : kGroups)) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    float L = 0.0f, M = kNegBig;
+    for (int i = i0 + (share ? lane : 0); i <= i1; i += share ? 64 : 1)
+      M = fmaxf(M, a.part_ml[2 * (part_at(a, hk, tile, i, i == i0 ? end0 : 0) + rr)]);
+    if (share) {
+#pragma unroll
+      for (int i = 32; i; i >>= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
+    }
+    for (int i = i0 + (share ? grp : 0); i <= i1; i += share ? kGroups : 1) {
+      const int64_t at = part_at(a, hk, tile, i, i == i0 ? end0 : 0) + rr;
+      const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_acc + at * D + d);
+      const float f = l == 0.0f ? 0.0f : fast_exp2(m - M);
+      if (l != 0.0f) v += f * x;                   // (else the part's keys are none of this row's)
+      L += f * l;
+    }
+    if (share) {
+      acc_s[tid] = v;
+      if (d == 0) l_s[grp] = L;
+      __syncthreads();
+      if (grp == 0) {
+        for (int i = 1; i < kGroups; ++i) {
+          v += acc_s[tid + i * (D / 4)];
+          L += l_s[i];
+        }
+      }
+      __syncthreads();
+    }
+    if (!share || grp == 0) {
+      const int row = row0 + rr, s = row / a.group;
+      store_row4<T>(a, b, hk * a.group + row - s * a.group, s, d, v, M, L);
     }
   }
 }

@@ -21,6 +21,7 @@ MI_DTYPE_F16 = 1
 MI_DTYPE_F32 = 2
 MI_STORE_SAME = 0
 MI_STORE_E4M3 = 1
+MI_PAGED_ATTN_MAX_SPLITS = 65536
 MI_OK = 0
 MI_ERR_INVALID = -1
 MI_ERR_UNSUPPORTED = -2
@@ -221,6 +222,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32, _i32, _i32, _ptr,                # dtype cdtype store stream
     ]),
     "mi_paged_attn_splits": (_i64, [_i64] * 7 + [_i32, _i32]),
+    "mi_paged_attn_workspace": (_i64, [_i64] * 6 + [_i32]),
     "mi_paged_attn": (_i32, [
         _ptr, _ptr, _ptr, _ptr,                # q k_pages v_pages scales
         _ptr, _ptr, _ptr, _ptr, _i64,          # page_table seq_lens query_lens part part_elems

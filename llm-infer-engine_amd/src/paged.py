@@ -246,7 +246,8 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
     keys j < seq_lens[b] - query_lens[b] + s + 1.  Tokens behind query_lens[b], and a
     token that sees no key, give 0.  out has q's strides; with ``return_lse`` also
     the fp32 log-sum-exp [B, n_heads, S] of the scaled scores (-inf for those).
-    ``num_splits``: key ranges per row (default: chosen from the CU count).
+    ``num_splits``: into how many parts a KV head's keys, those of all rows together, are
+    divided (default: chosen from the CU count; 1: no row is divided).
     """
     what = "paged_flash_attention"
     if q.dim() != 4:
@@ -266,8 +267,9 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
         raise ValueError(f"{what}: seq_lens must be given")
     seq_lens = _per_row(seq_lens, B, dev, "seq_lens", what)
     query_lens = _per_row(query_lens, B, dev, "query_lens", what)
-    if num_splits is not None and not 1 <= int(num_splits) <= 256:
-        raise ValueError(f"num_splits must be 1..256, got {num_splits}")
+    most = _lib.MI_PAGED_ATTN_MAX_SPLITS
+    if num_splits is not None and not 1 <= int(num_splits) <= most:
+        raise ValueError(f"num_splits must be 1..{most}, got {num_splits}")
     slots = page_table.shape[1]
     code = _lib.dtype_code(q.dtype)
     out = torch.empty_like(q)
@@ -285,7 +287,7 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
         num_splits = int(num_splits)
         part, n = None, 0
         if num_splits > 1:
-            n = B * H * S * num_splits * (D + 2)
+            n = lib.mi_paged_attn_workspace(B, H, cache.n_kv_heads, S, D, num_splits, code)
             part = torch.empty(n, device=dev, dtype=torch.float32)
         st = lib.mi_paged_attn(
             qs.data_ptr(), kp, vp, sp, page_table.data_ptr(), seq_lens.data_ptr(),

@@ -183,8 +183,10 @@ def test_c_append_refusals(over, code, msg):
 
 
 @pytest.mark.parametrize("over,code,msg", SHARED + [
-    ({"sl": None}, -1, "null"), ({"splits": 0}, -1, "num_splits"), ({"splits": 257}, -1, "num_splits"),
-    ({"splits": 2}, -1, "workspace"), ({"splits": 2, "part": P, "n": 2 * 4 * 66 - 1}, -1, "workspace"),
+    ({"sl": None}, -1, "null"), ({"splits": 0}, -1, "num_splits"), ({"splits": 65537}, -1, "num_splits"),
+    ({"splits": 2}, -1, "workspace"), ({"splits": 2, "part": P, "n": 2 * 2 * 2 * 16 * 66 - 1}, -1, "workspace"),
+    ({"splits": 2, "part": P + 4, "n": 1 << 30}, -1, "workspace"), ({"splits": 2, "dtype": 2, "part": P, "n": 2 * 4 * 66 - 1}, -1, "workspace"),
+    ({"B": 1 << 20, "slots": 1 << 22}, -2, "too many"),
     ({"kp": P + 8}, -1, "aligned"), ({"B": 1 << 20, "S": 1 << 20}, -2, "too many"),
 ])
 def test_c_attention_refusals(over, code, msg):
@@ -223,3 +225,5 @@ def test_workspace_and_split_questions_take_any_shape():
     for shape in ((0, 4, 2, 1, 64, 16, 4), (1, 4, 2, 1, 64, 0, 4), (1, 4, 2, 1, 64, 16, 1 << 62),
                   (1 << 40, 4, 2, 1, 64, 16, 4)):
         assert lib.mi_paged_attn_splits(*shape, 0, 1) == 1
+    for shape in ((0, 4, 2, 1, 64, 5), (1, 4, 2, 1, 64, 1), (1, 4, 3, 1, 64, 5), (1, 4, 2, 1, 512, 5)):
+        assert lib.mi_paged_attn_workspace(*shape, 0) == 0

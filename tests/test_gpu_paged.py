@@ -298,7 +298,7 @@ ATTEND = [
 
 
 @pytest.mark.parametrize("case", ATTEND, ids=lambda c: "-".join(str(x) for x in c[:7]))
-@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("splits", [None, 1, 7, 16])
 def test_attend_matches_oracle(dev, case, splits):
     dtype, store, Hq, Hkv, D, P, S, lens, qlens = case
     B = len(lens)
