@@ -33,7 +33,8 @@
 //
 // A load covers whole 128-byte lines where a key is one or more (a pair of loads takes
 // half-lines of its own rows and of rows 8 away, and the lanes exchange them), and is
-// non-temporal where no other block reads the same keys.
+// non-temporal where no other block reads the same keys.  A row of V longer than 64 bytes
+// is taken by two waves or steps, half a line each, and stays in the caches for the second.
 //
 // Keys behind the last visible one: their scores are -inf and their V entries are
 // zeroed, so that nothing in them (a NaN in an old page) reaches a sum.  Where
@@ -157,6 +158,7 @@ struct PagedWave {
   int Hkv, P, p_shift, slots;
   int lane, g, r;
   int lo, lim, minvis;        // keys [lo, lim); all rows that see any of them see [lo, minvis)
+  bool v_once;                // a step takes whole lines of V
   float scale_log2;
   Q8 q[R][D / 32];
   f32x4 o[R][D / 16];
@@ -237,7 +239,7 @@ struct PagedWave {
     const bool ok = chunk(key, pg.v, &at);
     const unsigned char* va = vp + at + (r * P + (key & (P - 1))) * G::ES;
 #pragma unroll
-    for (int i = 0; i < G::VL; ++i) st.v[i] = fetch(va + i * 16 * P * G::ES);
+    for (int i = 0; i < G::VL; ++i) st.v[i] = v_once ? fetch(va + i * 16 * P * G::ES) : load16(va + i * 16 * P * G::ES);
     st.scale = page_scale(pg.v, ok, 1);
   }
   // x for lanes of `banks` (0xc: r >= 8, 0x3: r < 8) from lane r ^ 8 of y
@@ -574,6 +576,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
   w.num_pages = (uint32_t)a.num_pages;
   w.Hkv = a.Hkv; w.P = a.P; w.p_shift = a.p_shift; w.slots = a.slots;
   w.scale_log2 = a.scale_log2;
+  w.v_once = a.P * G::ES <= 64;
 
   for (;;) {
     const RowKeys rk = row_keys(a, b);

@@ -15,15 +15,15 @@
 //
 // The choice compares sums over the vocabulary with a given number: between two
 // tokens the sums differ by one probability, 1e-5 and less in a flat row, which
-// sums of fp32 shares do not resolve.  Shares and sums are therefore fp64
-// (exp2_f64: a polynomial of 2^f to 1e-12, 17 instructions an element; the vector
-// units run fp64 at fp32's rate).
+// sums of fp32 shares do not resolve.  Sums are therefore fp64, and shares are good to
+// 1e-9 of themselves (Shares below: a table of 32 powers of two and a short fp32 series
+// for what is left).
 //
-// Three launches: `stats` reads every row that may matter once (chunks of 8192
+// Three launches: `stats` reads every row that may matter once (chunks of 8184
 // logits, each in its block's registers: largest value, its index, sum of shares
 // relative to it); `decide`, one block a (row, chunk), joins the stats, decides and
-// sums w over its chunk; `pick`, one block a row, finds the chunk and in it the
-// token.  T = 0 needs the first two only.
+// sums w over each wave's pieces of its chunk; `pick`, one wave a row, finds the piece
+// and in it the token.  T = 0 needs the first two only.
 #include <algorithm>
 
 #include "common.hpp"
@@ -46,7 +46,7 @@ struct VerifyArgs {
   double* sums;
   float* tops;
   int32_t* args;
-  double* wsum;       // [B, chunks, 2]: sums of w and of p
+  double* wsum;       // [B, chunks, pieces, 2]: sums of w and of p
   double* fin;        // [B, 4]: largest value and 1 / sum of row n, of the target and of the draft
   int64_t t_sb, t_ss, d_sb, d_ss, x_sb, x_ss, u_sb, u_ss;
   int64_t V;
@@ -54,33 +54,46 @@ struct VerifyArgs {
   int32_t B, S, rows, chunks, greedy;
 };
 
-// 2^y for y <= 0 to 1e-12 of its value: y = k + f, |f| <= 1/2, and the series of
-// e^(f ln 2) to the 10th power (the next term is below 3e-13).
-__device__ inline double exp2_f64(double y) {
-  y = fmax(y, -1100.0);            // 2^-1100 is 0
-  const double k = __builtin_rint(y);
-  const double t = (y - k) * 0.69314718055994530942;
-  double p = 1.0 / 3628800.0;
-  p = fma(p, t, 1.0 / 362880.0);
-  p = fma(p, t, 1.0 / 40320.0);
-  p = fma(p, t, 1.0 / 5040.0);
-  p = fma(p, t, 1.0 / 720.0);
-  p = fma(p, t, 1.0 / 120.0);
-  p = fma(p, t, 1.0 / 24.0);
-  p = fma(p, t, 1.0 / 6.0);
-  p = fma(p, t, 0.5);
-  p = fma(p, t, 1.0);
-  p = fma(p, t, 1.0);
-  return ldexp(p, (int)k);
+// Shares 2^((x - m) c) of logits x <= m.  y = (x - m) c in fp64; y = k / 32 + f, |f| <=
+// 1/64, k from the low bits of y + 1.5 * 2^47; 2^(k/32) is a table entry with k / 32's whole
+// part added to its exponent, 2^f = 1 + f p(f) with p the series of ln 2 (f ln 2)^i / (i+1)!
+// in fp32, off by 2^-24 of 0.011.  The table's 32 doubles lie on all 64 LDS banks once: no
+// lanes collide.
+struct Shares {
+  const double* table;      // LDS: 2^(i/32)
+  double c, mc;             // scale, m * scale
+  float m, lo;              // below lo a share is 0 (2^-1000)
+  __device__ inline void set(const double* t, float top, double scale) {
+    table = t;
+    m = top;
+    c = scale;
+    mc = (double)top * scale;
+    lo = top - (float)(1000.0 / scale);
+  }
+  __device__ inline double of(float x) const {
+    const bool in = x >= lo;
+    const double xd = (double)(in ? x : m);
+    const double magic = 211106232532992.0;         // 1.5 * 2^47
+    const double y = fma(xd, c, -mc), z = y + magic;
+    const int k = (int)__double_as_longlong(z);
+    const float f = (float)(y - (z - magic));
+    float p = 0.009618129f;                           // (ln 2)^4 / 4!
+    p = fmaf(p, f, 0.05550411f);                      // (ln 2)^3 / 3!
+    p = fmaf(p, f, 0.24022651f);                      // (ln 2)^2 / 2!
+    p = fmaf(p, f, 0.69314718f);
+    p *= f;
+    const double t = table[k & 31];
+    const double r = fma(t, (double)p, t);
+    const long long bits = __double_as_longlong(r) + ((long long)(k >> 5) << 52);
+    return in ? __longlong_as_double(bits) : 0.0;
+  }
+};
+__device__ inline void fill_table(double* t) {
+  if (threadIdx.x < 32) t[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
 }
 
 __device__ inline float logit(float x) {
   return x != x ? -INFINITY : fminf(x, 3.402823466e38f);
-}
-
-// share of a logit in a row whose largest is m (0 in a row without mass)
-__device__ inline double share(float x, float m, double c) {
-  return m == -INFINITY ? 0.0 : exp2_f64(((double)x - (double)m) * c);
 }
 
 __device__ inline int drafts_of(const VerifyArgs& a, int b) {
@@ -102,17 +115,25 @@ template <typename T>
 struct ChunkLogits {
   static constexpr int N = Chunk<T>::kN;       // logits of a group
   static constexpr int G = 32 / N;             // groups of a thread
+  static constexpr int kPieces = 4 * G;        // a wave's logits of one g: 64 N in a row
   float x[32];
   int64_t base;                                // place of group 0's first logit (may be < lo)
   __device__ inline int64_t place(int g) const { return base + ((int64_t)g * 256 + threadIdx.x) * N; }
   __device__ inline void load(const T* row, int64_t lo, int64_t hi) {
-    // the chunk starts at the group that holds lo
-    const int mis = (int)(((uintptr_t)(row + lo) % 16) / sizeof(T));
-    base = lo - mis;
+    base = first_place(row, lo);
+    load_places(row, lo, hi);
+  }
+  // the chunk starts at the group that holds lo
+  static __device__ inline int64_t first_place(const T* row, int64_t lo) {
+    return lo - (int64_t)(((uintptr_t)(row + lo) % 16) / sizeof(T));
+  }
+  // the logits at base's places (base may be another row's: groups are then not aligned)
+  __device__ inline void load_places(const T* row, int64_t lo, int64_t hi) {
+    const bool aligned = (uintptr_t)(row + base) % 16 == 0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const int64_t j = place(g);
-      if (j >= lo && j + N <= hi) {
+      if (aligned && j >= lo && j + N <= hi) {
         Chunk<T>::unpack(load16(row + j), x + g * N);
 #pragma unroll
         for (int e = 0; e < N; ++e) x[g * N + e] = logit(x[g * N + e]);
@@ -133,6 +154,8 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   __shared__ float top_s[4];
   __shared__ int64_t at_s[4];
   __shared__ double sum_s[4];
+  __shared__ double table[32];
+  fill_table(table);
   const int chunk = blockIdx.x, row = blockIdx.y % a.rows, b = blockIdx.y / a.rows;
   const int n = drafts_of(a, b);
   if (row <= a.S ? row > n : row - a.S - 1 >= n) return;   // no draft there
@@ -173,8 +196,10 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   }
   double sum = 0.0;
   if (!a.greedy && top > -INFINITY) {
+    Shares sh;
+    sh.set(table, top, a.c);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sum += exp2_f64(((double)c.x[i] - (double)top) * a.c);
+    for (int i = 0; i < 32; ++i) sum += sh.of(c.x[i]);
 #pragma unroll
     for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m, 64);
   }
@@ -188,26 +213,16 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   }
 }
 
-// the sum of a double over the block's 4 waves, in every thread
-__device__ inline double block_sum(double x, double* lds) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return lds[0] + lds[1] + lds[2] + lds[3];
-}
-
 // w and p of one logit pair of row n
 struct Weights {
-  float mt, md;
-  double zt, zd, c;
+  Shares t, d;
+  double zt, zd;
   bool refused, model;
   int64_t point;      // the drafted token of a refused draft without logits, else -1
-  __device__ inline void get(float t, float d, int64_t j, double* w, double* p) const {
-    *p = share(t, mt, c) * zt;
+  __device__ inline void get(float xt, float xd, int64_t j, double* w, double* p) const {
+    *p = t.m == -INFINITY ? 0.0 : t.of(xt) * zt;
     double q = 0.0;
-    if (refused) q = model ? share(d, md, c) * zd : (j == point ? 1.0 : 0.0);
+    if (refused) q = !model ? (j == point ? 1.0 : 0.0) : (d.m == -INFINITY ? 0.0 : d.of(xd) * zd);
     const double left = *p - q;
     *w = left > 0.0 ? left : 0.0;
   }
@@ -219,28 +234,46 @@ __global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
   __shared__ double inv_s[2 * kVMaxDrafts + 1];
   __shared__ int32_t arg_s[2 * kVMaxDrafts + 1];
   __shared__ int first_s;
-  __shared__ double red[4];
+  __shared__ double table[32];
   const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int n = drafts_of(a, b);
+  fill_table(table);
   if (tid == 0) first_s = n;
-  for (int row = tid; row < a.rows; row += 256) {
+  __syncthreads();
+  // 16 lanes join a row's chunks
+  const int l16 = tid & 15;
+  for (int row = tid >> 4; row < a.rows; row += 16) {
     if (row <= a.S ? row > n : row - a.S - 1 >= n) continue;
     const int64_t i = ((int64_t)b * a.rows + row) * a.chunks;
     float top = -INFINITY;
-    int32_t at = 0;
-    for (int c = 0; c < a.chunks; ++c) {
+    int32_t at = INT32_MAX;
+    for (int c = l16; c < a.chunks; c += 16) {
       const float t = a.tops[i + c];
       if (t > top) {
         top = t;
         at = a.args[i + c];
       }
     }
+#pragma unroll
+    for (int m = 8; m; m >>= 1) {
+      const float t2 = __shfl_xor(top, m, 16);
+      const int32_t a2 = __shfl_xor(at, m, 16);
+      at = t2 > top ? a2 : (t2 == top && a2 < at ? a2 : at);
+      top = fmaxf(top, t2);
+    }
     double z = 0.0;
-    if (!a.greedy)
-      for (int c = 0; c < a.chunks; ++c) z += share(a.tops[i + c], top, a.c) * a.sums[i + c];
-    top_s[row] = top;
-    arg_s[row] = top == -INFINITY ? -1 : at;
-    inv_s[row] = z > 0.0 ? 1.0 / z : 0.0;
+    if (!a.greedy && top > -INFINITY) {
+      Shares sh;
+      sh.set(table, top, a.c);
+      for (int c = l16; c < a.chunks; c += 16) z += sh.of(a.tops[i + c]) * a.sums[i + c];
+#pragma unroll
+      for (int m = 8; m; m >>= 1) z += __shfl_xor(z, m, 16);
+    }
+    if (l16 == 0) {
+      top_s[row] = top;
+      arg_s[row] = top == -INFINITY ? -1 : at;
+      inv_s[row] = z > 0.0 ? 1.0 / z : 0.0;
+    }
   }
   __syncthreads();
   const bool model = a.draft != nullptr;
@@ -250,13 +283,16 @@ __global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
     if (x >= 0 && x < a.V) {
       if (a.greedy) {
         ok = x == arg_s[tid];
-      } else {
-        const double p = share(logit(Elem<T>::to_f32(row_of<T>(a, b, tid)[x])), top_s[tid], a.c) *
-                         inv_s[tid];
+      } else if (top_s[tid] > -INFINITY) {
+        Shares sh;
+        sh.set(table, top_s[tid], a.c);
+        const double p = sh.of(logit(Elem<T>::to_f32(row_of<T>(a, b, tid)[x]))) * inv_s[tid];
         double q = 1.0;
+        const int dr = a.S + 1 + tid;
         if (model) {
-          const int dr = a.S + 1 + tid;
-          q = share(logit(Elem<T>::to_f32(row_of<T>(a, b, dr)[x])), top_s[dr], a.c) * inv_s[dr];
+          sh.set(table, top_s[dr], a.c);
+          q = top_s[dr] == -INFINITY
+                  ? 0.0 : sh.of(logit(Elem<T>::to_f32(row_of<T>(a, b, dr)[x]))) * inv_s[dr];
         }
         ok = (double)a.u[b * a.u_sb + tid * a.u_ss] * q < p;
       }
@@ -278,155 +314,166 @@ __global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
   Weights w;
   w.refused = k < n;
   w.model = model;
-  w.mt = top_s[k];
+  const int dr_row = a.S + 1 + k;
+  w.t.set(table, top_s[k], a.c);
   w.zt = inv_s[k];
-  w.md = w.refused && model ? top_s[a.S + 1 + k] : -INFINITY;
-  w.zd = w.refused && model ? inv_s[a.S + 1 + k] : 0.0;
-  w.c = a.c;
+  w.d.set(table, w.refused && model ? top_s[dr_row] : -INFINITY, a.c);
+  w.zd = w.refused && model ? inv_s[dr_row] : 0.0;
   w.point = w.refused && !model ? a.drafted[b * a.x_sb + k * a.x_ss] : -1;
   if (chunk == 0 && tid == 0) {
     double* f = a.fin + 4 * (int64_t)b;
-    f[0] = w.mt;
+    f[0] = w.t.m;
     f[1] = w.zt;
-    f[2] = w.md;
+    f[2] = w.d.m;
     f[3] = w.zd;
   }
   const int64_t lo = chunk * kVPlaces;
   const int64_t hi = lo + kVPlaces < a.V ? lo + kVPlaces : a.V;
-  const T* tr = row_of<T>(a, b, k);
-  const T* dr = w.refused && model ? row_of<T>(a, b, a.S + 1 + k) : nullptr;
-  double ws = 0.0, ps = 0.0;
-  if (dr != nullptr && ((uintptr_t)(tr + lo) - (uintptr_t)(dr + lo)) % 16 != 0) {
-    // rows of different alignment: one logit at a time
-    for (int64_t j = lo + tid; j < hi; j += 256) {
-      double wj, pj;
-      w.get(logit(Elem<T>::to_f32(tr[j])), logit(Elem<T>::to_f32(dr[j])), j, &wj, &pj);
-      ws += wj;
-      ps += pj;
-    }
-  } else {
-    ChunkLogits<T> ct, cd;
-    ct.load(tr, lo, hi);
-    if (dr != nullptr) cd.load(dr, lo, hi);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      double wj, pj;
-      w.get(ct.x[i], dr != nullptr ? cd.x[i] : -INFINITY, ct.place(i / ct.N) + i % ct.N, &wj, &pj);
-      ws += wj;
-      ps += pj;
-    }
+  ChunkLogits<T> ct, cd;
+  ct.load(row_of<T>(a, b, k), lo, hi);
+  const bool pair = w.refused && model;
+  if (pair) {
+    cd.base = ct.base;
+    cd.load_places(row_of<T>(a, b, dr_row), lo, hi);
   }
-  ws = block_sum(ws, red);
-  ps = block_sum(ps, red);
-  if (tid == 0) {
-    a.wsum[2 * ((int64_t)b * a.chunks + chunk)] = ws;
-    a.wsum[2 * ((int64_t)b * a.chunks + chunk) + 1] = ps;
+  double* out = a.wsum + 2 * ((int64_t)b * a.chunks + chunk) * ct.kPieces;
+#pragma unroll
+  for (int g = 0; g < ct.G; ++g) {
+    double ws = 0.0, ps = 0.0;
+#pragma unroll
+    for (int e = 0; e < ct.N; ++e) {
+      const int i = g * ct.N + e;
+      double wj, pj;
+      w.get(ct.x[i], pair ? cd.x[i] : -INFINITY, ct.place(g) + e, &wj, &pj);
+      ws += wj;
+      ps += pj;
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) {
+      ws += __shfl_xor(ws, m, 64);
+      ps += __shfl_xor(ps, m, 64);
+    }
+    if ((tid & 63) == 0) {
+      out[2 * (4 * g + (tid >> 6))] = ws;
+      out[2 * (4 * g + (tid >> 6)) + 1] = ps;
+    }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double pre_s[256];
-  __shared__ double below_s;
-  __shared__ int chunk_s;
-  __shared__ long long hit_s, last_s;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int n = drafts_of(a, b), k = (int)a.accepted[b];
-  const double* sums = a.wsum + 2 * (int64_t)b * a.chunks;
-  double total = 0.0, total_p = 0.0;
-  for (int c = 0; c < a.chunks; ++c) {
-    total += sums[2 * c];
-    total_p += sums[2 * c + 1];
+// inclusive sums over the wave's lanes
+__device__ inline double wave_scan(double x, int lane) {
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const double y = __shfl_up(x, i, 64);
+    if (lane >= i) x += y;
   }
-  const bool use_w = total > 0.0;              // else p itself (also where nothing was refused: w is p)
-  if (!use_w) total = total_p;
+  return x;
+}
+
+// One wave a row.  The pieces' sums, a run of them for each lane, lead to the piece in
+// which the sum passes the goal; its 64 N logits, N a lane, to the token.  (Should
+// rounding pass the goal nowhere, the last place with mass is taken.)
+template <typename T>
+__global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
+  typedef ChunkLogits<T> C;
+  __shared__ double table[32];
+  const int b = blockIdx.x, lane = threadIdx.x;
+  fill_table(table);
+  __syncthreads();
+  const int n = drafts_of(a, b), k = (int)a.accepted[b];
+  const int64_t n_pieces = (int64_t)a.chunks * C::kPieces;
+  const double* sums = a.wsum + 2 * (int64_t)b * n_pieces;
+  const int64_t per = (n_pieces + 63) / 64;
+  const int64_t i0 = lane * per < n_pieces ? lane * per : n_pieces;
+  const int64_t i1 = i0 + per < n_pieces ? i0 + per : n_pieces;
+  double ws = 0.0, ps = 0.0;
+  for (int64_t i = i0; i < i1; ++i) {
+    ws += sums[2 * i];
+    ps += sums[2 * i + 1];
+  }
+  const double ws_end = wave_scan(ws, lane), ps_end = wave_scan(ps, lane);
+  const double total_w = __shfl(ws_end, 63, 64), total_p = __shfl(ps_end, 63, 64);
+  // w, or p itself where w is zero everywhere (where nothing was refused w is p)
+  const bool use_w = total_w > 0.0;
+  const double total = use_w ? total_w : total_p;
+  int64_t* out = a.tokens + (int64_t)b * (a.S + 1) + k;
+  if (!(total > 0.0)) {                        // a row without mass: no token
+    if (lane == 0) *out = -1;
+    return;
+  }
   const double goal = (double)a.r[b] * total;
-  if (tid == 0) {
-    // the chunk in which the sum passes the goal; the last one with mass, should rounding pass none
-    double run = 0.0, below = 0.0;
-    int at = -1;
-    for (int c = 0; c < a.chunks; ++c) {
-      const double x = sums[2 * c + (use_w ? 0 : 1)];
+  const double mine = use_w ? ws : ps, mine_end = use_w ? ws_end : ps_end;
+  uint64_t over = __ballot(mine > 0.0 && mine_end > goal);
+  if (over == 0) over = 1ull << (63 - __builtin_clzll(__ballot(mine > 0.0)));
+  const int who = (int)__builtin_ctzll(over);
+  int64_t piece = -1;
+  double below = 0.0;
+  if (lane == who) {
+    double run = mine_end - mine;
+    for (int64_t i = i0; i < i1; ++i) {
+      const double x = sums[2 * i + (use_w ? 0 : 1)];
       if (x > 0.0) {
-        at = c;
+        piece = i;
         below = run;
         if (run + x > goal) break;
       }
       run += x;
     }
-    chunk_s = at;
-    below_s = below;
-    hit_s = INT64_MAX;
-    last_s = -1;
   }
-  __syncthreads();
-  int64_t* out = a.tokens + (int64_t)b * (a.S + 1) + k;
-  if (chunk_s < 0) {                           // a row without mass: no token
-    if (tid == 0) *out = -1;
-    return;
-  }
+  piece = __shfl((long long)piece, who, 64);
+  below = __shfl(below, who, 64);
+
   Weights w;
   const double* f = a.fin + 4 * (int64_t)b;
   w.refused = k < n;
   w.model = a.draft != nullptr;
-  w.mt = (float)f[0];
+  w.t.set(table, (float)f[0], a.c);
   w.zt = f[1];
-  w.md = (float)f[2];
+  w.d.set(table, (float)f[2], a.c);
   w.zd = f[3];
-  w.c = a.c;
   w.point = w.refused && !w.model ? a.drafted[b * a.x_sb + k * a.x_ss] : -1;
   const T* tr = row_of<T>(a, b, k);
   const T* dr = w.refused && w.model ? row_of<T>(a, b, a.S + 1 + k) : nullptr;
-  const int64_t lo = chunk_s * kVPlaces;
+  const int64_t lo = piece / C::kPieces * kVPlaces;
   const int64_t hi = lo + kVPlaces < a.V ? lo + kVPlaces : a.V;
-  // 32 places in a row for each thread, their sum, the sums before them, then the place
-  const int64_t j0 = lo + 32 * tid;
-  double mine = 0.0;
-  for (int e = 0; e < 32; ++e) {
+  const int64_t j0 = C::first_place(tr, lo) + (piece % C::kPieces * 64 + lane) * C::N;
+  double x[C::N], sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < C::N; ++e) {
     const int64_t j = j0 + e;
-    if (j >= hi) break;
-    double wj, pj;
-    w.get(logit(Elem<T>::to_f32(tr[j])), dr != nullptr ? logit(Elem<T>::to_f32(dr[j])) : -INFINITY, j, &wj, &pj);
-    mine += use_w ? wj : pj;
-  }
-  pre_s[tid] = mine;
-  __syncthreads();
-  for (int s = 1; s < 256; s <<= 1) {          // inclusive sums over the threads
-    const double x = tid >= s ? pre_s[tid - s] : 0.0;
-    __syncthreads();
-    pre_s[tid] += x;
-    __syncthreads();
-  }
-  double run = below_s + (tid > 0 ? pre_s[tid - 1] : 0.0);
-  if (mine > 0.0) {
-    const bool over = below_s + pre_s[tid] > goal;
-    long long last = -1;
-    for (int e = 0; e < 32; ++e) {
-      const int64_t j = j0 + e;
-      if (j >= hi) break;
+    x[e] = 0.0;
+    if (j >= lo && j < hi) {
       double wj, pj;
-      w.get(logit(Elem<T>::to_f32(tr[j])), dr != nullptr ? logit(Elem<T>::to_f32(dr[j])) : -INFINITY, j, &wj, &pj);
-      const double x = use_w ? wj : pj;
-      run += x;
-      if (x > 0.0) {
-        last = j;
-        if (over && run > goal) {
-          atomicMin((unsigned long long*)&hit_s, (unsigned long long)j);
-          break;
-        }
-      }
+      w.get(logit(Elem<T>::to_f32(tr[j])), dr != nullptr ? logit(Elem<T>::to_f32(dr[j])) : -INFINITY, j,
+            &wj, &pj);
+      x[e] = use_w ? wj : pj;
     }
-    // (the sums of one place after the other may end a rounding below the thread's sum)
-    if (over) atomicMin((unsigned long long*)&hit_s, (unsigned long long)last);
-    atomicMax(&last_s, last);
+    sum += x[e];
   }
-  __syncthreads();
-  if (tid == 0) *out = hit_s != INT64_MAX ? hit_s : last_s;
+  double run = below + wave_scan(sum, lane) - sum;
+  int64_t hit = INT64_MAX, last = -1;
+#pragma unroll
+  for (int e = 0; e < C::N; ++e) {
+    run += x[e];
+    if (x[e] > 0.0) {
+      last = j0 + e;
+      if (run > goal && hit == INT64_MAX) hit = j0 + e;
+    }
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) {
+    const int64_t h = __shfl_xor((long long)hit, m, 64), l = __shfl_xor((long long)last, m, 64);
+    hit = h < hit ? h : hit;
+    last = l > last ? l : last;
+  }
+  if (lane == 0) *out = hit != INT64_MAX ? hit : last;
 }
 
 namespace {
 
 int64_t verify_chunks(int64_t vocab) { return (vocab + kVPlaces - 1) / kVPlaces; }
+// pieces of a chunk: 16 for 2-byte logits, 32 for fp32
+int64_t verify_pieces(int64_t vocab) { return verify_chunks(vocab) * 32; }
 int64_t up8(int64_t bytes) { return (bytes + 7) / 8 * 8; }
 
 template <typename T>
@@ -434,7 +481,7 @@ void launch_verify(const VerifyArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(verify_stats_kernel<T>, dim3(a.chunks, a.B * a.rows), dim3(256), 0, st, a);
   hipLaunchKernelGGL(verify_decide_kernel<T>, dim3(a.greedy ? 1 : a.chunks, a.B), dim3(256), 0, st, a);
   if (!a.greedy)
-    hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(a.B), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(verify_pick_kernel<T>, dim3(a.B), dim3(64), 0, st, a);
 }
 
 }  // namespace
@@ -447,7 +494,7 @@ extern "C" int64_t mi_verify_drafts_workspace(int64_t batch, int64_t drafts, int
       vocab > INT32_MAX)
     return 0;
   const int64_t chunks = verify_chunks(vocab), cells = batch * (2 * drafts + 1) * chunks;
-  return 8 * cells + up8(4 * cells) + up8(4 * cells) + 16 * batch * chunks + 32 * batch;
+  return 8 * cells + up8(4 * cells) + up8(4 * cells) + 16 * batch * verify_pieces(vocab) + 32 * batch;
 }
 
 extern "C" int32_t mi_verify_drafts(
@@ -500,7 +547,7 @@ extern "C" int32_t mi_verify_drafts(
   const int64_t cells = batch * a.rows * a.chunks;
   char* w = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<double*>(w); w += 8 * cells;
-  a.wsum = reinterpret_cast<double*>(w); w += 16 * batch * a.chunks;
+  a.wsum = reinterpret_cast<double*>(w); w += 16 * batch * verify_pieces(vocab);
   a.fin = reinterpret_cast<double*>(w); w += 32 * batch;
   a.tops = reinterpret_cast<float*>(w); w += up8(4 * cells);
   a.args = reinterpret_cast<int32_t*>(w);
