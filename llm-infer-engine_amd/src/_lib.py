@@ -322,13 +322,10 @@ class _Here:
 _HERE = _Here()
 
 
-def on_device_of(t: torch.Tensor):
-    """Context in which t's device is the current one, for launches and for the
+def on_device(index: int):
+    """Context in which device `index` is the current one, for launches and for the
     library's questions about the current device."""
-    index = t.get_device()
-    if index < 0 or index == torch._C._cuda_getDevice():
-        return _HERE
-    return torch.cuda.device(index)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 _ARRIVE: dict[tuple[int, int], int | None] = {}

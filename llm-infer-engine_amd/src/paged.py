@@ -101,10 +101,8 @@ class PagedKVCache:
             raise ValueError(f"{what}: layer_idx {layer_idx} out of range for a cache of {n} layers")
         i = layer_idx % n
         k, v, s = self.k, self.v, self.scales
-        if not (k.is_cuda and v.is_cuda):
-            raise ValueError(f"{what} requires CUDA tensors")
-        return (k.data_ptr() + i * k.stride(0) * k.element_size(),
-                v.data_ptr() + i * v.stride(0) * v.element_size(),
+        es = k.element_size()
+        return (k.data_ptr() + i * k.stride(0) * es, v.data_ptr() + i * v.stride(0) * es,
                 None if s is None else s.data_ptr() + 4 * i * s.stride(0))
 
 
@@ -122,28 +120,44 @@ def _check_pages(dtype, kv_dtype, num_pages, page_size, head_dim):
         raise ValueError(f"PagedKVCache: head_dim must be even and at most 256, got {head_dim}")
 
 
-def _per_row(t, batch: int, device, name: str, what: str):
+_I32, _I64 = torch.int32, torch.int64
+
+
+def _per_row(t, batch: int, index: int, name: str, what: str):
     """A device int64 [batch] tensor of row lengths or positions (None stays None)."""
     if t is None:
         return None
-    if t.dim() != 1 or t.shape[0] != batch:
+    if t.shape != (batch,):
         raise ValueError(f"{what}: {name} must have shape ({batch},), got {tuple(t.shape)}")
-    if t.dtype != torch.int64 or t.device != device or t.stride(0) != 1:
+    if t.dtype is not _I64 or t.get_device() != index or t.stride(0) != 1:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise TypeError(f"{what}: {name} must hold integers, got {t.dtype}")
+        device = torch.device("cpu") if index < 0 else torch.device("cuda", index)
         t = t.to(device=device, dtype=torch.int64).contiguous()
     return t
 
 
-def _table(page_table, batch: int, device, what: str):
+def _table(page_table, batch: int, index: int, what: str):
     if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1:
         raise ValueError(f"{what}: page_table must have shape ({batch}, slots), got "
                          f"{tuple(page_table.shape)}")
-    if page_table.dtype != torch.int32:
+    if page_table.dtype is not _I32:
         raise TypeError(f"{what}: page_table must have dtype torch.int32, got {page_table.dtype}")
-    if page_table.device != device:
-        raise ValueError(f"{what}: page_table must be on {device}, got {page_table.device}")
+    if page_table.get_device() != index:
+        raise ValueError(f"{what}: page_table must be on device {index}, got {page_table.device}")
     return page_table if page_table.stride(1) == 1 else page_table.contiguous()
+
+
+def _device_of(what: str, *tensors) -> int:
+    """The index of the one CUDA device that all of them are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            if not all(x.is_cuda for x in tensors):
+                raise ValueError(f"{what} requires CUDA tensors")
+            raise ValueError(f"{what}: all tensors must be on one device, got "
+                             f"{', '.join(sorted({str(x.device) for x in tensors}))}")
+    return index
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -177,7 +191,6 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
     if xk.dim() != 4 or xv.shape != xk.shape:
         raise ValueError(f"xk and xv shapes must match, got {tuple(xk.shape)} and {tuple(xv.shape)}")
     B, Hkv, S, D = xk.shape
-    dev = xk.device
     if Hkv != cache.n_kv_heads or D != cache.head_dim:
         raise ValueError(f"xk/xv shape {tuple(xk.shape)} does not fit a cache of "
                          f"{cache.n_kv_heads} heads of {cache.head_dim}")
@@ -189,25 +202,21 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
             raise ValueError(f"xq shape {tuple(xq.shape)} does not match xk {tuple(xk.shape)}")
         _check_heads(xq, cache, Hkv, what)
         H = xq.shape[1]
-    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or rope_cos.shape[1] < D // 2:
+    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or 2 * rope_cos.shape[1] < D:
         raise ValueError(f"{what}: cos/sin must be 2-D [positions, head_dim // 2 = {D // 2}], got "
                          f"{tuple(rope_cos.shape)} and {tuple(rope_sin.shape)}")
     if rope_cos.dtype != rope_sin.dtype or rope_cos.dtype not in (xk.dtype, torch.float32):
         raise TypeError(f"{what}: cos/sin must have dtype {xk.dtype} or float32, got "
                         f"{rope_cos.dtype} and {rope_sin.dtype}")
     kp, vp, sp = cache._layer(layer_idx, what)
-    for t in (xk, xv, rope_cos, rope_sin, cache.k, *(() if xq is None else (xq,))):
-        if not t.is_cuda:
-            raise ValueError(f"{what} requires CUDA tensors")
-        if t.device != dev:
-            raise ValueError(f"{what}: all tensors must be on {dev}, got one on {t.device}")
-    page_table = _table(page_table, B, dev, what)
+    index = _device_of(what, xk, xv, rope_cos, rope_sin, cache.k, xk if xq is None else xq)
+    page_table = _table(page_table, B, index, what)
     first, start = 0, None
     if isinstance(start_pos, torch.Tensor):
-        start = _per_row(start_pos, B, dev, "start_pos", what)
+        start = _per_row(start_pos, B, index, "start_pos", what)
     else:
         first = int(start_pos)
-    query_lens = _per_row(query_lens, B, dev, "query_lens", what)
+    query_lens = _per_row(query_lens, B, index, "query_lens", what)
     xk, xv = _rows(xk), _rows(xv)
     if rope_cos.stride(1) != 1 or rope_sin.stride(1) != 1:
         rope_cos, rope_sin = rope_cos.contiguous(), rope_sin.contiguous()
@@ -216,11 +225,11 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
     if xq is not None:
         out = torch.empty_like(xq)
         qs = _rows(xq)
-        dst = out if out.stride(3) == 1 else torch.empty(xq.shape, dtype=xq.dtype, device=dev)
+        dst = out if out.stride(3) == 1 else torch.empty(xq.shape, dtype=xq.dtype, device=xq.device)
         q_strides, o_strides = qs.stride()[:3], dst.stride()[:3]
     if B == 0 or S == 0:
         return out
-    with _lib.on_device_of(xk):
+    with _lib.on_device(index):
         st = _lib.load().mi_rope_paged_append(
             _lib.ptr(qs), xk.data_ptr(), xv.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
             _lib.ptr(dst), kp, vp, sp, page_table.data_ptr(), first, _lib.ptr(start),
@@ -228,7 +237,7 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
             cache.page_size, page_table.shape[1], *q_strides, *xk.stride()[:3],
             *xv.stride()[:3], *o_strides, page_table.stride(0), rope_cos.stride(0),
             rope_sin.stride(0), _lib.dtype_code(xk.dtype), _lib.dtype_code(rope_cos.dtype),
-            cache.store, _lib.stream_of(xk))
+            cache.store, torch._C._cuda_getCurrentRawStream(index))
     _lib.check(st, what)
     if dst is not out:
         out.copy_(dst)
@@ -253,34 +262,29 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
     if q.dim() != 4:
         raise ValueError("q must be a rank-4 tensor")
     B, H, S, D = q.shape
-    dev = q.device
     if D != cache.head_dim:
         raise ValueError(f"q head_dim {D} does not fit a cache of head_dim {cache.head_dim}")
     _check_heads(q, cache, cache.n_kv_heads, what)
-    if not q.is_cuda:
-        raise ValueError(f"{what} requires CUDA tensors")
     kp, vp, sp = cache._layer(layer_idx, what)
-    if cache.k.device != dev:
-        raise ValueError(f"{what}: q is on {dev}, the cache on {cache.k.device}")
-    page_table = _table(page_table, B, dev, what)
+    index = _device_of(what, q, cache.k)
+    page_table = _table(page_table, B, index, what)
     if seq_lens is None:
         raise ValueError(f"{what}: seq_lens must be given")
-    seq_lens = _per_row(seq_lens, B, dev, "seq_lens", what)
-    query_lens = _per_row(query_lens, B, dev, "query_lens", what)
-    most = _lib.MI_PAGED_ATTN_MAX_SPLITS
-    if num_splits is not None and not 1 <= int(num_splits) <= most:
-        raise ValueError(f"num_splits must be 1..{most}, got {num_splits}")
+    seq_lens = _per_row(seq_lens, B, index, "seq_lens", what)
+    query_lens = _per_row(query_lens, B, index, "query_lens", what)
+    if num_splits is not None and not 1 <= int(num_splits) <= _lib.MI_PAGED_ATTN_MAX_SPLITS:
+        raise ValueError(f"num_splits must be 1..{_lib.MI_PAGED_ATTN_MAX_SPLITS}, got {num_splits}")
     slots = page_table.shape[1]
     code = _lib.dtype_code(q.dtype)
     out = torch.empty_like(q)
-    lse = torch.empty((B, H, S), device=dev, dtype=torch.float32) if return_lse else None
+    lse = torch.empty((B, H, S), device=q.device, dtype=torch.float32) if return_lse else None
     if B == 0 or S == 0:
         return (out, lse) if return_lse else out
     lib = _lib.load()
     qs = _rows(q)
-    dst = out if out.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dst = out if out.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    with _lib.on_device_of(q):
+    with _lib.on_device(index):
         if num_splits is None:
             num_splits = lib.mi_paged_attn_splits(B, H, cache.n_kv_heads, S, D, cache.page_size,
                                                   slots, code, cache.store)
@@ -288,13 +292,13 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
         part, n = None, 0
         if num_splits > 1:
             n = lib.mi_paged_attn_workspace(B, H, cache.n_kv_heads, S, D, num_splits, code)
-            part = torch.empty(n, device=dev, dtype=torch.float32)
+            part = torch.empty(n, device=q.device, dtype=torch.float32)
         st = lib.mi_paged_attn(
             qs.data_ptr(), kp, vp, sp, page_table.data_ptr(), seq_lens.data_ptr(),
             _lib.ptr(query_lens), _lib.ptr(part), n, dst.data_ptr(), _lib.ptr(lse), B, H,
             cache.n_kv_heads, S, D, cache.num_pages, cache.page_size, slots, num_splits,
             *qs.stride()[:3], *dst.stride()[:3], page_table.stride(0), scale, code, cache.store,
-            _lib.stream_of(q))
+            torch._C._cuda_getCurrentRawStream(index))
     _lib.check(st, what)
     if dst is not out:
         out.copy_(dst)

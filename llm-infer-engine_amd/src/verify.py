@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .paged import _per_row
+from .paged import _device_of, _per_row
 
 
 def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
@@ -42,7 +42,6 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
                          f"{tuple(target_logits.shape)} and {tuple(draft_tokens.shape)}")
     B, S = draft_tokens.shape
     V = target_logits.shape[2]
-    dev = target_logits.device
     if target_logits.shape[:2] != (B, S + 1):
         raise ValueError(f"{what}: target_logits {tuple(target_logits.shape)} must have {S + 1} rows "
                          f"for each of the {B} rows of drafts")
@@ -71,14 +70,9 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
         if draft_logits.dtype != target_logits.dtype:
             raise TypeError(f"{what}: draft_logits dtype {draft_logits.dtype} must match "
                             f"target_logits {target_logits.dtype}")
-    for t in (target_logits, draft_tokens, accept_u, sample_u, draft_logits):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{what} requires CUDA tensors")
-        if t.device != dev:
-            raise ValueError(f"{what}: all tensors must be on {dev}, got one on {t.device}")
-    draft_lens = _per_row(draft_lens, B, dev, "draft_lens", what)
+    index = _device_of(what, *[t for t in (target_logits, draft_tokens, accept_u, sample_u,
+                                           draft_logits) if t is not None])
+    draft_lens = _per_row(draft_lens, B, index, "draft_lens", what)
     if target_logits.stride(2) != 1:
         target_logits = target_logits.contiguous()
     if draft_logits is not None and draft_logits.stride(2) != 1:
@@ -86,13 +80,13 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
     if sample_u is not None and sample_u.stride(0) != 1:
         sample_u = sample_u.contiguous()
     lib = _lib.load()
-    tokens = torch.empty((B, S + 1), device=dev, dtype=torch.int64)
-    accepted = torch.empty((B,), device=dev, dtype=torch.int64)
+    tokens = torch.empty((B, S + 1), device=target_logits.device, dtype=torch.int64)
+    accepted = torch.empty((B,), device=target_logits.device, dtype=torch.int64)
     if B == 0:
         return tokens, accepted
     n = lib.mi_verify_drafts_workspace(B, S, V)
-    ws = torch.empty(max(n, 8), device=dev, dtype=torch.uint8)   # (0: refused by the call)
-    with _lib.on_device_of(target_logits):
+    ws = torch.empty(max(n, 8), device=target_logits.device, dtype=torch.uint8)   # (0: refused by the call)
+    with _lib.on_device(index):
         st = lib.mi_verify_drafts(
             target_logits.data_ptr(), _lib.ptr(draft_logits), draft_tokens.data_ptr(),
             _lib.ptr(accept_u), _lib.ptr(sample_u), _lib.ptr(draft_lens), tokens.data_ptr(),
@@ -100,6 +94,6 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
             target_logits.stride(0), target_logits.stride(1),
             *((0, 0) if draft_logits is None else draft_logits.stride()[:2]),
             *draft_tokens.stride(), *((0, 0) if accept_u is None else accept_u.stride()),
-            temperature, code, _lib.stream_of(target_logits))
+            temperature, code, torch._C._cuda_getCurrentRawStream(index))
     _lib.check(st, what)
     return tokens, accepted

@@ -100,7 +100,7 @@ def test_attention_refusals(over, exc, msg):
 
 def test_row_and_table_checks():
     from src import paged
-    dev = torch.device("cpu")
+    dev = -1   # the device index of host tensors
     with pytest.raises(ValueError, match="shape"):
         paged._per_row(torch.zeros(2, dtype=torch.int64), 3, dev, "seq_lens", "f")
     with pytest.raises(TypeError, match="integers"):
