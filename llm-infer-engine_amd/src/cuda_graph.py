@@ -33,6 +33,7 @@ import torch.nn as nn
 
 from .config import ModelArgs
 from .kv_cache import KVCache
+from .paged import PagedKVCache
 
 
 def _accepts(fn, name: str) -> bool:
@@ -48,6 +49,9 @@ class CUDAGraphDecodeRunner:
                  *, batch_size: int | None = None, greedy: bool = False):
         if not str(device).startswith("cuda"):
             raise ValueError("CUDAGraphDecodeRunner requires CUDA device")
+        if isinstance(kv_cache, PagedKVCache):
+            raise ValueError("CUDAGraphDecodeRunner steps a KVCache; capture a paged forward with "
+                             "torch.cuda.graph (its lengths and page table are device tensors)")
         self.model = model
         self.model_args = model_args
         self.kv_cache = kv_cache

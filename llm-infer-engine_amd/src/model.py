@@ -15,6 +15,10 @@ Extensions (keyword-only, defaults keep the reference behaviour):
     the device position, so a replay copies nothing from the host.
   * ``greedy=True`` returns (logits, tokens): tokens [B, 1] int64 is the
     argmax of the returned logits, computed on the device.
+  * a ``PagedKVCache`` (src/paged.py) with ``page_table`` [B, slots], and with
+    ``start_positions`` / ``query_lens`` [B] (device int64) where rows start at
+    their own positions or have fewer tokens: prompts, pieces of prompts, drafts
+    and single tokens alike append to the rows' pages and attend over them.
 The final norm and the output projection of up to 16 rows (decode, or the
 last position of a prefill) run as one fused launch (src/lm_head.py).
 """
@@ -26,6 +30,7 @@ import torch.nn as nn
 from . import lm_head
 from .flash_attn import flash_attention
 from .flash_decode import flash_decode
+from .paged import PagedKVCache, paged_flash_attention, rope_and_paged_update
 from .rms_norm import RMSNorm
 from .rope import (
     DeviceRopeTable,
@@ -77,7 +82,8 @@ class Attention(nn.Module):
 
     def forward(self, x, rope_cos, rope_sin, layer_idx=None, start_pos=0, kv_cache=None,
                 use_cuda_graph=False, scatter_positions=None, decode_attn_mask=None, *,
-                seq_lens=None, rope_by_position=False, residual=None):
+                seq_lens=None, rope_by_position=False, residual=None,
+                page_table=None, start_positions=None, query_lens=None):
         batch_size, query_len, _ = x.shape
         torch.cuda.nvtx.range_push("QKV_proj")
         xq, xk, xv = self.qkv(x)
@@ -85,6 +91,20 @@ class Attention(nn.Module):
         xq = xq.view(batch_size, query_len, self.n_heads, self.head_dim).transpose(1, 2)
         xk = xk.view(batch_size, query_len, self.n_kv_heads, self.head_dim).transpose(1, 2)
         xv = xv.view(batch_size, query_len, self.n_kv_heads, self.head_dim).transpose(1, 2)
+
+        if isinstance(kv_cache, PagedKVCache):
+            # rope_cos / rope_sin are full tables here, seq_lens counts the new tokens too
+            torch.cuda.nvtx.range_push("KV_cache")
+            if layer_idx is None or page_table is None:
+                raise ValueError("layer_idx and page_table are required when using a PagedKVCache")
+            xq = rope_and_paged_update(xk, xv, rope_cos, rope_sin, kv_cache, layer_idx, page_table,
+                                       start_positions, query_lens=query_lens, xq=xq)
+            torch.cuda.nvtx.range_pop()
+            torch.cuda.nvtx.range_push("FlashAttn")
+            output = paged_flash_attention(xq, kv_cache, layer_idx, page_table, seq_lens,
+                                           query_lens=query_lens)
+            torch.cuda.nvtx.range_pop()
+            return self._project(output, batch_size, query_len, residual)
 
         positions = scatter_positions if (use_cuda_graph and scatter_positions is not None) else None
         q_positions = positions if rope_by_position else None
@@ -114,6 +134,9 @@ class Attention(nn.Module):
             output = flash_decode(xq, xk, xv, mask=decode_attn_mask, seq_lens=seq_lens)
             torch.cuda.nvtx.range_pop()
 
+        return self._project(output, batch_size, query_len, residual)
+
+    def _project(self, output, batch_size, query_len, residual):
         torch.cuda.nvtx.range_push("Output_proj")
         output = output.transpose(1, 2).contiguous().view(batch_size, query_len, -1)
         out = self.out_proj(output, residual)
@@ -175,9 +198,34 @@ class Llama3(nn.Module):
             self._rope_table = t
         return t
 
+    def _paged_rows(self, tokens, start_pos, page_table, start_positions, query_lens, **other):
+        """Start positions and key counts (new tokens included) of a paged forward's rows."""
+        given = [name for name, value in other.items() if value is not None]
+        if given:
+            raise ValueError(f"a PagedKVCache takes page_table, start_positions and query_lens, "
+                             f"not {', '.join(given)}")
+        if page_table is None:
+            raise ValueError("page_table is required when using a PagedKVCache")
+        B, S = tokens.shape
+        if start_positions is None:
+            start_positions = torch.full((B,), int(start_pos), dtype=torch.int64,
+                                         device=tokens.device)
+        return start_positions, start_positions + (S if query_lens is None else query_lens.clamp(0, S))
+
     def forward(self, tokens, start_pos=0, kv_cache=None, freqs_cis=None, use_cuda_graph=False,
                 scatter_positions=None, decode_attn_mask=None, return_all_logits=False, *,
-                seq_lens=None, greedy=False):
+                seq_lens=None, greedy=False, page_table=None, start_positions=None,
+                query_lens=None):
+        ext = {}
+        paged = isinstance(kv_cache, PagedKVCache)
+        if paged:
+            start_positions, seq_lens = self._paged_rows(
+                tokens, start_pos, page_table, start_positions, query_lens, freqs_cis=freqs_cis,
+                scatter_positions=scatter_positions, decode_attn_mask=decode_attn_mask,
+                seq_lens=seq_lens)
+            ext = dict(page_table=page_table, start_positions=start_positions, query_lens=query_lens)
+        elif page_table is not None or start_positions is not None or query_lens is not None:
+            raise ValueError("page_table, start_positions and query_lens need a PagedKVCache")
         torch.cuda.nvtx.range_push("Embed")
         # the same rows as self.tok_embeddings(tokens); the indexing gather loads
         # every element at once (a decode step's 8 rows: 2.2 us in a hipGraph
@@ -186,7 +234,7 @@ class Llama3(nn.Module):
         torch.cuda.nvtx.range_pop()
         seq_len = tokens.shape[1]
         by_pos = bool(use_cuda_graph and scatter_positions is not None and freqs_cis is None)
-        if by_pos:
+        if by_pos or paged:
             table = self.rope_table(h.dtype, h.device)
             rope_cos, rope_sin = table.cos, table.sin
         elif freqs_cis is None:
@@ -199,11 +247,15 @@ class Llama3(nn.Module):
             h = layer(h, rope_cos, rope_sin, layer_idx=layer_idx, start_pos=start_pos,
                       kv_cache=kv_cache, use_cuda_graph=use_cuda_graph,
                       scatter_positions=scatter_positions, decode_attn_mask=decode_attn_mask,
-                      seq_lens=seq_lens, rope_by_position=by_pos)
+                      seq_lens=seq_lens, rope_by_position=by_pos, **ext)
         torch.cuda.nvtx.range_pop()
         torch.cuda.nvtx.range_push("Output")
         if not return_all_logits and seq_len > 1:
-            h = h[:, -1:, :]
+            if query_lens is not None:   # a row's last token that is real
+                last = (query_lens - 1).clamp(0, seq_len - 1).to(h.device)
+                h = h[torch.arange(h.shape[0], device=h.device), last][:, None]
+            else:
+                h = h[:, -1:, :]
         rows = h.shape[0] * h.shape[1]
         if h.is_cuda and lm_head.supported(rows, h.shape[-1], self.output.weight, self.norm.weight):
             # final norm + output projection (+ greedy argmax) in one launch

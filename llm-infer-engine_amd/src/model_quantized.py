@@ -23,6 +23,7 @@ from torch.nn.modules import module as _hooks
 from . import decode_layer, quant_linear
 from .flash_decode import flash_decode
 from .model import Attention, FeedForward, Llama3, TransformerBlock
+from .paged import PagedKVCache
 from .quant_linear import W8A16Linear
 from .quant_utils import quantize_weight_symmetric_per_channel
 
@@ -183,6 +184,8 @@ class QuantizedTransformerBlock(TransformerBlock):
         the cache and where no module's call is observed or replaced."""
         if not self.fused_decode or kv_cache is None or layer_idx is None or x.shape[1] != 1:
             return None
+        if isinstance(kv_cache, PagedKVCache):
+            return None  # the fused launch appends to a dense cache
         if positions is not None and not rope_by_position:
             return None  # per-step sliced tables at a device position: op chain
         attn, ff = self.attention, self.feed_forward
