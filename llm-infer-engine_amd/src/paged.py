@@ -85,6 +85,8 @@ class PagedKVCache:
         self.n_layers, self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         self.kv_dtype = k.dtype
         self.store = _lib.MI_STORE_SAME if scales is None else _lib.MI_STORE_E4M3
+        self._code = _lib.dtype_code(dtype)
+        self._layer_bytes = k.stride(0) * k.element_size()
 
     def reset(self):
         """Empty pages (zeros).  Not needed before a page is used again: its first
@@ -99,11 +101,10 @@ class PagedKVCache:
         n = self.n_layers
         if not -n <= layer_idx < n:
             raise ValueError(f"{what}: layer_idx {layer_idx} out of range for a cache of {n} layers")
-        i = layer_idx % n
-        k, v, s = self.k, self.v, self.scales
-        es = k.element_size()
-        return (k.data_ptr() + i * k.stride(0) * es, v.data_ptr() + i * v.stride(0) * es,
-                None if s is None else s.data_ptr() + 4 * i * s.stride(0))
+        i, s = layer_idx % n, self.scales
+        at = i * self._layer_bytes
+        return (self.k.data_ptr() + at, self.v.data_ptr() + at,
+                None if s is None else s.data_ptr() + 8 * i * self.num_pages * self.n_kv_heads)
 
 
 def _check_pages(dtype, kv_dtype, num_pages, page_size, head_dim):
@@ -123,29 +124,36 @@ def _check_pages(dtype, kv_dtype, num_pages, page_size, head_dim):
 _I32, _I64 = torch.int32, torch.int64
 
 
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+
+
 def _per_row(t, batch: int, index: int, name: str, what: str):
     """A device int64 [batch] tensor of row lengths or positions (None stays None)."""
     if t is None:
         return None
     if t.shape != (batch,):
         raise ValueError(f"{what}: {name} must have shape ({batch},), got {tuple(t.shape)}")
-    if t.dtype is not _I64 or t.get_device() != index or t.stride(0) != 1:
-        if t.is_floating_point() or t.dtype == torch.bool:
-            raise TypeError(f"{what}: {name} must hold integers, got {t.dtype}")
-        device = torch.device("cpu") if index < 0 else torch.device("cuda", index)
-        t = t.to(device=device, dtype=torch.int64).contiguous()
-    return t
+    if t.dtype is _I64 and t.get_device() == index and t.stride() == (1,):
+        return t
+    if t.is_floating_point() or t.dtype == torch.bool:
+        raise TypeError(f"{what}: {name} must hold integers, got {t.dtype}")
+    device = torch.device("cpu") if index < 0 else torch.device("cuda", index)
+    return t.to(device=device, dtype=torch.int64).contiguous()
 
 
 def _table(page_table, batch: int, index: int, what: str):
-    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1:
-        raise ValueError(f"{what}: page_table must have shape ({batch}, slots), got "
-                         f"{tuple(page_table.shape)}")
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != batch or shape[1] < 1:
+        raise ValueError(f"{what}: page_table must have shape ({batch}, slots), got {tuple(shape)}")
     if page_table.dtype is not _I32:
         raise TypeError(f"{what}: page_table must have dtype torch.int32, got {page_table.dtype}")
     if page_table.get_device() != index:
         raise ValueError(f"{what}: page_table must be on device {index}, got {page_table.device}")
-    return page_table if page_table.stride(1) == 1 else page_table.contiguous()
+    stride = page_table.stride()
+    if stride[1] != 1:
+        page_table = page_table.contiguous()
+        stride = page_table.stride()
+    return page_table, shape[1], stride[0]
 
 
 def _device_of(what: str, *tensors) -> int:
@@ -153,24 +161,20 @@ def _device_of(what: str, *tensors) -> int:
     index = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != index or index < 0:
-            if not all(x.is_cuda for x in tensors):
-                raise ValueError(f"{what} requires CUDA tensors")
-            raise ValueError(f"{what}: all tensors must be on one device, got "
-                             f"{', '.join(sorted({str(x.device) for x in tensors}))}")
-    return index
+            break
+    else:
+        return index
+    if not all(x.is_cuda for x in tensors):
+        raise ValueError(f"{what} requires CUDA tensors")
+    raise ValueError(f"{what}: all tensors must be on one device, got "
+                     f"{', '.join(sorted({str(x.device) for x in tensors}))}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with unit head_dim stride."""
-    return t if t.stride(3) == 1 else t.contiguous()
-
-
-def _check_heads(q, cache, n_kv_heads, what):
-    if q.shape[1] % n_kv_heads != 0:
-        raise ValueError(f"query heads ({q.shape[1]}) must be divisible by KV heads ({n_kv_heads})")
-    if q.dtype != cache.dtype:
-        raise TypeError(f"{what}: q dtype {q.dtype} must match the cache's activations "
-                        f"{cache.dtype}")
+def _check_heads(H, dtype, cache, what):
+    if H % cache.n_kv_heads != 0:
+        raise ValueError(f"query heads ({H}) must be divisible by KV heads ({cache.n_kv_heads})")
+    if dtype is not cache.dtype:
+        raise TypeError(f"{what}: q dtype {dtype} must match the cache's activations {cache.dtype}")
 
 
 def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer_idx: int,
@@ -188,57 +192,73 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
     Returns the rotated xq (with xq's strides), or None.
     """
     what = "rope_and_paged_update"
-    if xk.dim() != 4 or xv.shape != xk.shape:
-        raise ValueError(f"xk and xv shapes must match, got {tuple(xk.shape)} and {tuple(xv.shape)}")
-    B, Hkv, S, D = xk.shape
+    shape, dtype = xk.shape, xk.dtype
+    if len(shape) != 4 or xv.shape != shape:
+        raise ValueError(f"xk and xv shapes must match, got {tuple(shape)} and {tuple(xv.shape)}")
+    B, Hkv, S, D = shape
     if Hkv != cache.n_kv_heads or D != cache.head_dim:
-        raise ValueError(f"xk/xv shape {tuple(xk.shape)} does not fit a cache of "
-                         f"{cache.n_kv_heads} heads of {cache.head_dim}")
-    if xk.dtype != cache.dtype or xv.dtype != cache.dtype:
-        raise TypeError(f"xk/xv dtype {xk.dtype} must match the cache's activations {cache.dtype}")
+        raise ValueError(f"xk/xv shape {tuple(shape)} does not fit a cache of {cache.n_kv_heads} "
+                         f"heads of {cache.head_dim}")
+    if dtype is not cache.dtype or xv.dtype is not dtype:
+        raise TypeError(f"xk/xv dtype {dtype} must match the cache's activations {cache.dtype}")
     H = Hkv
     if xq is not None:
-        if xq.dim() != 4 or xq.shape[0] != B or xq.shape[2] != S or xq.shape[3] != D:
-            raise ValueError(f"xq shape {tuple(xq.shape)} does not match xk {tuple(xk.shape)}")
-        _check_heads(xq, cache, Hkv, what)
-        H = xq.shape[1]
-    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or 2 * rope_cos.shape[1] < D:
+        q_shape = xq.shape
+        if len(q_shape) != 4 or q_shape[0] != B or q_shape[2] != S or q_shape[3] != D:
+            raise ValueError(f"xq shape {tuple(q_shape)} does not match xk {tuple(shape)}")
+        H = q_shape[1]
+        _check_heads(H, xq.dtype, cache, what)
+    t_shape, t_dtype = rope_cos.shape, rope_cos.dtype
+    if len(t_shape) != 2 or rope_sin.shape != t_shape or 2 * t_shape[1] < D:
         raise ValueError(f"{what}: cos/sin must be 2-D [positions, head_dim // 2 = {D // 2}], got "
-                         f"{tuple(rope_cos.shape)} and {tuple(rope_sin.shape)}")
-    if rope_cos.dtype != rope_sin.dtype or rope_cos.dtype not in (xk.dtype, torch.float32):
-        raise TypeError(f"{what}: cos/sin must have dtype {xk.dtype} or float32, got "
-                        f"{rope_cos.dtype} and {rope_sin.dtype}")
+                         f"{tuple(t_shape)} and {tuple(rope_sin.shape)}")
+    if rope_sin.dtype is not t_dtype or (t_dtype is not dtype and t_dtype is not _F32):
+        raise TypeError(f"{what}: cos/sin must have dtype {dtype} or float32, got {t_dtype} and "
+                        f"{rope_sin.dtype}")
     kp, vp, sp = cache._layer(layer_idx, what)
     index = _device_of(what, xk, xv, rope_cos, rope_sin, cache.k, xk if xq is None else xq)
-    page_table = _table(page_table, B, index, what)
+    page_table, slots, pt_stride = _table(page_table, B, index, what)
     first, start = 0, None
     if isinstance(start_pos, torch.Tensor):
         start = _per_row(start_pos, B, index, "start_pos", what)
     else:
         first = int(start_pos)
-    query_lens = _per_row(query_lens, B, index, "query_lens", what)
-    xk, xv = _rows(xk), _rows(xv)
-    if rope_cos.stride(1) != 1 or rope_sin.stride(1) != 1:
+    lens = _per_row(query_lens, B, index, "query_lens", what)
+    ks, vs, cs, ss = xk.stride(), xv.stride(), rope_cos.stride(), rope_sin.stride()
+    if ks[3] != 1:
+        xk = xk.contiguous()
+        ks = xk.stride()
+    if vs[3] != 1:
+        xv = xv.contiguous()
+        vs = xv.stride()
+    if cs[1] != 1 or ss[1] != 1:
         rope_cos, rope_sin = rope_cos.contiguous(), rope_sin.contiguous()
-    out = dst = qs = None
-    q_strides = o_strides = (0, 0, 0)
+        cs, ss = rope_cos.stride(), rope_sin.stride()
+    out = dst = q_ptr = o_ptr = None
+    qs = os_ = (0, 0, 0, 1)
     if xq is not None:
-        out = torch.empty_like(xq)
-        qs = _rows(xq)
-        dst = out if out.stride(3) == 1 else torch.empty(xq.shape, dtype=xq.dtype, device=xq.device)
-        q_strides, o_strides = qs.stride()[:3], dst.stride()[:3]
+        out = dst = torch.empty_like(xq)
+        qs, os_ = xq.stride(), out.stride()
+        if qs[3] != 1:
+            xq = xq.contiguous()
+            qs = xq.stride()
+        if os_[3] != 1:
+            dst = torch.empty(q_shape, dtype=dtype, device=out.device)
+            os_ = dst.stride()
+        q_ptr, o_ptr = xq.data_ptr(), dst.data_ptr()
     if B == 0 or S == 0:
         return out
     with _lib.on_device(index):
         st = _lib.load().mi_rope_paged_append(
-            _lib.ptr(qs), xk.data_ptr(), xv.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
-            _lib.ptr(dst), kp, vp, sp, page_table.data_ptr(), first, _lib.ptr(start),
-            _lib.ptr(query_lens), rope_cos.shape[0], B, H, Hkv, S, D, cache.num_pages,
-            cache.page_size, page_table.shape[1], *q_strides, *xk.stride()[:3],
-            *xv.stride()[:3], *o_strides, page_table.stride(0), rope_cos.stride(0),
-            rope_sin.stride(0), _lib.dtype_code(xk.dtype), _lib.dtype_code(rope_cos.dtype),
-            cache.store, torch._C._cuda_getCurrentRawStream(index))
-    _lib.check(st, what)
+            q_ptr, xk.data_ptr(), xv.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), o_ptr,
+            kp, vp, sp, page_table.data_ptr(), first, None if start is None else start.data_ptr(),
+            None if lens is None else lens.data_ptr(),
+            t_shape[0], B, H, Hkv, S, D, cache.num_pages, cache.page_size, slots,
+            qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os_[0], os_[1], os_[2],
+            pt_stride, cs[0], ss[0], cache._code, _lib.dtype_code(t_dtype), cache.store,
+            torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _lib.check(st, what)
     if dst is not out:
         out.copy_(dst)
     return out
@@ -259,47 +279,53 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
     divided (default: chosen from the CU count; 1: no row is divided).
     """
     what = "paged_flash_attention"
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("q must be a rank-4 tensor")
-    B, H, S, D = q.shape
+    B, H, S, D = shape
     if D != cache.head_dim:
         raise ValueError(f"q head_dim {D} does not fit a cache of head_dim {cache.head_dim}")
-    _check_heads(q, cache, cache.n_kv_heads, what)
+    _check_heads(H, q.dtype, cache, what)
     kp, vp, sp = cache._layer(layer_idx, what)
     index = _device_of(what, q, cache.k)
-    page_table = _table(page_table, B, index, what)
+    page_table, slots, pt_stride = _table(page_table, B, index, what)
     if seq_lens is None:
         raise ValueError(f"{what}: seq_lens must be given")
     seq_lens = _per_row(seq_lens, B, index, "seq_lens", what)
-    query_lens = _per_row(query_lens, B, index, "query_lens", what)
+    lens = _per_row(query_lens, B, index, "query_lens", what)
     if num_splits is not None and not 1 <= int(num_splits) <= _lib.MI_PAGED_ATTN_MAX_SPLITS:
         raise ValueError(f"num_splits must be 1..{_lib.MI_PAGED_ATTN_MAX_SPLITS}, got {num_splits}")
-    slots = page_table.shape[1]
-    code = _lib.dtype_code(q.dtype)
-    out = torch.empty_like(q)
-    lse = torch.empty((B, H, S), device=q.device, dtype=torch.float32) if return_lse else None
+    out = dst = torch.empty_like(q)
+    lse = q.new_empty((B, H, S), dtype=_F32) if return_lse else None
     if B == 0 or S == 0:
         return (out, lse) if return_lse else out
-    lib = _lib.load()
-    qs = _rows(q)
-    dst = out if out.stride(3) == 1 else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    qs, os_ = q.stride(), out.stride()
+    if qs[3] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    if os_[3] != 1:
+        dst = torch.empty(shape, dtype=q.dtype, device=q.device)
+        os_ = dst.stride()
+    lib, code, Hkv = _lib.load(), cache._code, cache.n_kv_heads
     with _lib.on_device(index):
         if num_splits is None:
-            num_splits = lib.mi_paged_attn_splits(B, H, cache.n_kv_heads, S, D, cache.page_size,
-                                                  slots, code, cache.store)
+            num_splits = lib.mi_paged_attn_splits(B, H, Hkv, S, D, cache.page_size, slots, code,
+                                                  cache.store)
         num_splits = int(num_splits)
         part, n = None, 0
         if num_splits > 1:
-            n = lib.mi_paged_attn_workspace(B, H, cache.n_kv_heads, S, D, num_splits, code)
-            part = torch.empty(n, device=q.device, dtype=torch.float32)
+            n = lib.mi_paged_attn_workspace(B, H, Hkv, S, D, num_splits, code)
+            part = q.new_empty((n,), dtype=_F32)
         st = lib.mi_paged_attn(
-            qs.data_ptr(), kp, vp, sp, page_table.data_ptr(), seq_lens.data_ptr(),
-            _lib.ptr(query_lens), _lib.ptr(part), n, dst.data_ptr(), _lib.ptr(lse), B, H,
-            cache.n_kv_heads, S, D, cache.num_pages, cache.page_size, slots, num_splits,
-            *qs.stride()[:3], *dst.stride()[:3], page_table.stride(0), scale, code, cache.store,
+            q.data_ptr(), kp, vp, sp, page_table.data_ptr(), seq_lens.data_ptr(),
+            None if lens is None else lens.data_ptr(), None if part is None else part.data_ptr(),
+            n, dst.data_ptr(), None if lse is None else lse.data_ptr(), B, H, Hkv, S, D,
+            cache.num_pages, cache.page_size, slots, num_splits, qs[0], qs[1], qs[2],
+            os_[0], os_[1], os_[2], pt_stride,
+            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), code, cache.store,
             torch._C._cuda_getCurrentRawStream(index))
-    _lib.check(st, what)
+    if st:
+        _lib.check(st, what)
     if dst is not out:
         out.copy_(dst)
     return (out, lse) if return_lse else out

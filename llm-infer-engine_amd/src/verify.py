@@ -80,20 +80,21 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
     if sample_u is not None and sample_u.stride(0) != 1:
         sample_u = sample_u.contiguous()
     lib = _lib.load()
-    tokens = torch.empty((B, S + 1), device=target_logits.device, dtype=torch.int64)
-    accepted = torch.empty((B,), device=target_logits.device, dtype=torch.int64)
+    # (int64, on the device: tokens, counts and the workspace's 8-byte words)
+    tokens, accepted = draft_tokens.new_empty((B, S + 1)), draft_tokens.new_empty((B,))
     if B == 0:
         return tokens, accepted
     n = lib.mi_verify_drafts_workspace(B, S, V)
-    ws = torch.empty(max(n, 8), device=target_logits.device, dtype=torch.uint8)   # (0: refused by the call)
+    ws = draft_tokens.new_empty((n // 8 + 1,))
+    ts, xs = target_logits.stride(), draft_tokens.stride()
+    ds = (0, 0) if draft_logits is None else draft_logits.stride()
+    us = (0, 0) if accept_u is None else accept_u.stride()
     with _lib.on_device(index):
         st = lib.mi_verify_drafts(
             target_logits.data_ptr(), _lib.ptr(draft_logits), draft_tokens.data_ptr(),
             _lib.ptr(accept_u), _lib.ptr(sample_u), _lib.ptr(draft_lens), tokens.data_ptr(),
-            accepted.data_ptr(), ws.data_ptr(), n, B, S, V,
-            target_logits.stride(0), target_logits.stride(1),
-            *((0, 0) if draft_logits is None else draft_logits.stride()[:2]),
-            *draft_tokens.stride(), *((0, 0) if accept_u is None else accept_u.stride()),
-            temperature, code, torch._C._cuda_getCurrentRawStream(index))
-    _lib.check(st, what)
+            accepted.data_ptr(), ws.data_ptr(), n, B, S, V, ts[0], ts[1], ds[0], ds[1],
+            xs[0], xs[1], us[0], us[1], temperature, code, torch._C._cuda_getCurrentRawStream(index))
+    if st:
+        _lib.check(st, what)
     return tokens, accepted
