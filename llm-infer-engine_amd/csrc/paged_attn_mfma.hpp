@@ -502,9 +502,21 @@ __device__ inline int parts_used(int total, int parts) {
   const int most = (total + 3) >> 2;
   return most < parts ? most : parts;
 }
-__device__ inline int part_start(int i, int total, int used) {
-  return (int)((int64_t)i * total / used);
-}
+// part i takes q or, the first ones, q + 1 units of total = used * q + more
+struct Parts {
+  int used, q, more;
+  __device__ inline Parts(int total, int parts) {
+    used = parts_used(total, parts);
+    q = used > 0 ? total / used : 0;
+    more = total - q * used;
+  }
+  __device__ inline int start(int i) const { return i * q + (i < more ? i : more); }
+  // the part that holds unit x
+  __device__ inline int of(int x) const {
+    const int longer = more * (q + 1);
+    return x < longer ? x / (q + 1) : more + (x - longer) / q;
+  }
+};
 // workspace: sums (D floats) and m, l of the two ends of each part
 __device__ inline int64_t part_at(const PagedAttnArgs& a, int hk, int tile, int part, int end) {
   return ((((int64_t)hk * a.tiles + tile) * a.parts + part) * 2 + end) * a.kv_rows;
@@ -553,10 +565,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
   int b = part, u = 0, u1 = 0, row_u = 0;
   if (a.parts > 0) {
     const int total = list.total();
-    const int used = parts_used(total, a.parts);
-    if (part >= used) return;
-    u = part_start(part, total, used);
-    u1 = part_start(part + 1, total, used);
+    const Parts parts(total, a.parts);
+    if (part >= parts.used) return;
+    u = parts.start(part);
+    u1 = parts.start(part + 1);
     while (list.held_end() <= u) list.hold(list.b0 + 64, list.held_end());
     const int at = (int)__builtin_ctzll(__ballot(list.end > u));
     b = list.b0 + at;
@@ -595,6 +607,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
     w.minvis = rk.vis(list.s_first);
     w.minvis = w.minvis > w.lo ? w.minvis : w.lo;
     w.table = a.table + (int64_t)b * a.t_sb;
+    // page numbers first: they are on their way while q is loaded
+    constexpr int kStride = 4 * G::STEP;
+    int base = w.lo + wave * G::STEP;
+    typename Wave::Pages pg = w.lookup(base), next = w.lookup(base + kStride);
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
       const int row = row0 + 16 * rt + w.r;
@@ -624,10 +640,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
       }
     }
 
-    int base = w.lo + wave * G::STEP;
     if (base < hi) {
-      constexpr int kStride = 4 * G::STEP;
-      typename Wave::Pages pg = w.lookup(base), next = w.lookup(base + kStride);
       typename Wave::VStep v;
       if constexpr (PagedAhead<E8, D, R>::value) {
         // K of the next step is on its way from before this step's products, V of the next
@@ -754,15 +767,14 @@ __global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
   const int units = __builtin_amdgcn_readlane(list.units, b - list.b0);
   const int first_u = end - units;
   const int grp = tid / (D / 4), d = 4 * (tid % (D / 4));
-  // the part that holds unit x is the last one that starts at x or before
-  const int used = parts_used(total, a.parts);
+  const Parts parts(total, a.parts);
   int i0 = 0, i1 = -1, end0 = 0;
   if (units > 0) {
-    i0 = (int)((((int64_t)first_u + 1) * used - 1) / total);
-    i1 = (int)(((int64_t)end * used - 1) / total);
+    i0 = parts.of(first_u);
+    i1 = parts.of(end - 1);
     if (i0 == i1) return;
     // (in part i0 the row is the last one, unless it starts with it; in the others the first)
-    end0 = part_start(i0, total, used) == first_u ? 0 : 1;
+    end0 = parts.start(i0) == first_u ? 0 : 1;
   }
   const bool share = i1 - i0 >= 4;
   for (int rr = blockIdx.y + (share ? 0 : (int)gridDim.y * grp); rr < rows;
