@@ -543,8 +543,9 @@ int64_t mi_lm_head_partials(int64_t m, int64_t n);
  * already holds earlier positions keeps at least its scale, and its earlier entries
  * are rounded again to a larger one.  A value that is not finite is stored as NaN.
  * Unit head_dim strides; rows of xq [batch, n_heads, seq_len, head_dim], xk and xv
- * [batch, n_kv_heads, ..]; cdtype = dtype or fp32.  Rows whose newest page is the
- * same page, or a position twice in a call, leave one of the writers' values.
+ * [batch, n_kv_heads, ..]; cdtype = dtype or fp32.  Rows may share pages that they
+ * only read.  Two rows that append to one page, or a page twice among the slots that
+ * a row appends to, leave its entries undefined (nothing else is touched).
  * The paged form of mi_rope and mi_rope_kv_append (src/rope.py:94-119, :255-313).
  */
 int32_t mi_rope_paged_append(
@@ -564,7 +565,7 @@ int32_t mi_rope_paged_append(
  * own.  out [batch, n_heads, seq_len, head_dim] in q's dtype, lse (optional fp32
  * [batch, n_heads, seq_len], natural log); a query that sees no key, and the rows
  * behind query_lens[b], give 0 and -inf.  Keys behind seq_lens[b] are not counted,
- * whatever their memory holds.  Scores, softmax and sums are fp32.
+ * whatever their memory holds.  Scores, softmax and sums are fp32; sm_scale > 0.
  * num_splits: 1, a row's keys are not divided (one launch); 2..
  * MI_PAGED_ATTN_MAX_SPLITS, the keys of a KV head, those of all rows together, are
  * divided into so many parts, which needs `part`, 16-byte aligned, of

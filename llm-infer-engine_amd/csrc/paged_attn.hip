@@ -298,6 +298,10 @@ extern "C" int32_t mi_paged_attn(
                    (long long)num_splits);
     return MI_ERR_INVALID;
   }
+  if (!(sm_scale > 0.0f) || sm_scale > 3.402823466e38f) {
+    set_last_error("paged_attn: sm_scale must be positive and finite");
+    return MI_ERR_INVALID;
+  }
   if ((uintptr_t)k_pages % 16 != 0 || (uintptr_t)v_pages % 16 != 0) {
     set_last_error("paged_attn: pages must be 16-byte aligned");
     return MI_ERR_INVALID;

@@ -331,7 +331,8 @@ struct PagedWave {
         }
       }
     }
-    const float c = E8 ? st.scale * scale_log2 : scale_log2;
+    // (not below the least normal number: -inf times it must stay -inf)
+    const float c = fmaxf(E8 ? st.scale * scale_log2 : scale_log2, 1.17549435e-38f);
     // every row sees all keys of the step, and their pages exist
     whole = base + G::STEP <= minvis && __all(here);
     if (!whole) {

@@ -187,7 +187,8 @@ def rope_and_paged_update(xk, xv, rope_cos, rope_sin, cache: PagedKVCache, layer
     rope_sin [positions, head_dim // 2] (in xk's dtype or fp32; the nearest row
     outside them).  With ``query_lens`` (device int64 [B]) only a row's first
     query_lens[b] tokens are appended.  Positions behind the table's slots, before 0 or
-    in slots without a page are not written.
+    in slots without a page are not written.  Rows may share pages that they only read;
+    a page that two rows append to holds undefined entries.
 
     Returns the rotated xq (with xq's strides), or None.
     """
@@ -295,6 +296,9 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
     lens = _per_row(query_lens, B, index, "query_lens", what)
     if num_splits is not None and not 1 <= int(num_splits) <= _lib.MI_PAGED_ATTN_MAX_SPLITS:
         raise ValueError(f"num_splits must be 1..{_lib.MI_PAGED_ATTN_MAX_SPLITS}, got {num_splits}")
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{what}: sm_scale must be positive and finite, got {sm_scale}")
     out = dst = torch.empty_like(q)
     lse = q.new_empty((B, H, S), dtype=_F32) if return_lse else None
     if B == 0 or S == 0:
@@ -321,8 +325,7 @@ def paged_flash_attention(q, cache: PagedKVCache, layer_idx: int, page_table, se
             None if lens is None else lens.data_ptr(), None if part is None else part.data_ptr(),
             n, dst.data_ptr(), None if lse is None else lse.data_ptr(), B, H, Hkv, S, D,
             cache.num_pages, cache.page_size, slots, num_splits, qs[0], qs[1], qs[2],
-            os_[0], os_[1], os_[2], pt_stride,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), code, cache.store,
+            os_[0], os_[1], os_[2], pt_stride, scale, code, cache.store,
             torch._C._cuda_getCurrentRawStream(index))
     if st:
         _lib.check(st, what)

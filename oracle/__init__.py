@@ -21,6 +21,9 @@ How each part is pinned (see tests/test_oracle_*.py):
   quant               hand-built rows (zeros, ties, +-amax), |q| <= 127.
   linear              integer-exact cases computed with Python ints.
   norm                constant-row closed form.
+  paged               the dense attention and append on the same tokens, e4m3's own
+                      table of values, the scale's defining inequality, hand-computed
+                      acceptances; a key too many fails the bar.
   model               transformers' LlamaForCausalLM (fp32, CPU) on the same
                       checkpoint, token by token: logits within 1e-4 of scale,
                       bf16 and W8A16 weights, default and llama3 RoPE, tied and

@@ -155,12 +155,12 @@ def c_append(**o):
 def c_attn(**o):
     from src import _lib
     a = dict(q=P, kp=P, vp=P, sc=None, pt=P, sl=P, ql=None, part=None, n=0, out=P, lse=None, B=1, Hq=4,
-             Hkv=2, S=1, D=64, pages=8, page=16, slots=4, splits=1, dtype=0, store=0)
+             Hkv=2, S=1, D=64, pages=8, page=16, slots=4, splits=1, dtype=0, store=0, scale=0.125)
     a.update(o)
     return _lib.load().mi_paged_attn(
         a["q"], a["kp"], a["vp"], a["sc"], a["pt"], a["sl"], a["ql"], a["part"], a["n"], a["out"],
         a["lse"], a["B"], a["Hq"], a["Hkv"], a["S"], a["D"], a["pages"], a["page"], a["slots"],
-        a["splits"], *[64] * 6, 4, 0.125, a["dtype"], a["store"], None)
+        a["splits"], *[64] * 6, 4, a["scale"], a["dtype"], a["store"], None)
 
 
 SHARED = [
@@ -187,7 +187,8 @@ def test_c_append_refusals(over, code, msg):
     ({"splits": 2}, -1, "workspace"), ({"splits": 2, "part": P, "n": 2 * 2 * 2 * 16 * 66 - 1}, -1, "workspace"),
     ({"splits": 2, "part": P + 4, "n": 1 << 30}, -1, "workspace"), ({"splits": 2, "dtype": 2, "part": P, "n": 2 * 4 * 66 - 1}, -1, "workspace"),
     ({"B": 1 << 20, "slots": 1 << 22}, -2, "too many"),
-    ({"kp": P + 8}, -1, "aligned"), ({"B": 1 << 20, "S": 1 << 20}, -2, "too many"),
+    ({"scale": 0.0}, -1, "sm_scale"), ({"scale": -1.0}, -1, "sm_scale"), ({"scale": float("nan")}, -1, "sm_scale"),
+    ({"scale": float("inf")}, -1, "sm_scale"), ({"kp": P + 8}, -1, "aligned"), ({"B": 1 << 20, "S": 1 << 20}, -2, "too many"),
 ])
 def test_c_attention_refusals(over, code, msg):
     from src import _lib

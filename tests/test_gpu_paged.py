@@ -409,6 +409,46 @@ def test_attend_layouts_and_scale(dev, dtype, store, D):
         assert torch.equal(paged_flash_attention(x, *args), plain)
 
 
+@pytest.mark.parametrize("sm_scale", [0.0, -0.1, float("nan"), float("inf")])
+def test_attend_refuses_scales(dev, sm_scale):
+    from src.paged import paged_flash_attention
+    cache = cache_of(dev, *make_pages(2, 2, 16, 64, BF16, "same", 118), BF16)
+    with pytest.raises(ValueError, match="sm_scale"):
+        paged_flash_attention(randn((1, 4, 1, 64), 119, device=dev), cache, 0,
+                              torch.zeros((1, 2), dtype=torch.int32, device=dev),
+                              torch.ones(1, dtype=torch.int64, device=dev), sm_scale=sm_scale)
+
+
+@pytest.mark.parametrize("exp", [-120, 90])
+def test_attend_pages_of_extreme_scales(dev, exp):
+    """Pages whose scales are near the ends of what a page can have (K and V; the other is
+    ordinary): scores that vanish, values near fp32's ends."""
+    k, v, sc = make_pages(6, 2, 32, 64, BF16, "e4m3", 115)
+    q, table, lens = randn((2, 4, 2, 64), 116), table_of(2, 3, 6, 117), [90, 65]
+    for which in ((0, 1) if exp < 0 else (1,)):
+        s = sc.clone()
+        s[..., which] = 2.0 ** exp
+        check_attend(dev, q, k, v, s, table, lens, dtype=BF16)
+
+
+def test_attend_rows_share_pages(dev):
+    """Rows with the same first pages (a shared prefix), and a page twice in one row."""
+    k, v, sc = make_pages(8, 2, 16, 128, F16, "e4m3", 113)
+    table = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5], [6, 6, 6, 0]], dtype=torch.int32)
+    check_attend(dev, randn((3, 4, 2, 128), 114, F16), k, v, sc, table, [60, 49, 50], dtype=F16)
+
+
+@pytest.mark.parametrize("B,splits", [(70, None), (130, 300), (200, 3)])
+def test_attend_many_rows(dev, B, splits):
+    """More rows than a wave has lanes, most of them empty or short."""
+    P, slots = 16, 6
+    k, v, sc = make_pages(40, 1, P, 64, BF16, "e4m3", 123)
+    g = torch.Generator().manual_seed(124)
+    table = torch.randint(0, 40, (B, slots), generator=g).int()
+    lens = [0 if i % 3 == 0 else (5 * i) % (P * slots + 1) for i in range(B)]
+    check_attend(dev, randn((B, 2, 1, 64), 125), k, v, sc, table, lens, dtype=BF16, num_splits=splits)
+
+
 def test_attend_empty_calls(dev):
     from src.paged import paged_flash_attention
     k, v, sc = make_pages(4, 2, 16, 64, BF16, "e4m3", 120)
