@@ -788,13 +788,25 @@ __global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int i = 32; i; i >>= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
     }
-    for (int i = i0 + (share ? grp : 0); i <= i1; i += share ? kGroups : 1) {
-      const int64_t at = part_at(a, hk, tile, i, i == i0 ? end0 : 0) + rr;
-      const float m = a.part_ml[2 * at], l = a.part_ml[2 * at + 1];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_acc + at * D + d);
-      const float f = l == 0.0f ? 0.0f : fast_exp2(m - M);
-      if (l != 0.0f) v += f * x;                   // (else the part's keys are none of this row's)
-      L += f * l;
+    // 4 parts' loads in flight at a time
+    const int step = share ? kGroups : 1;
+    for (int i = i0 + (share ? grp : 0); i <= i1; i += 4 * step) {
+      float m[4], l[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = i + j * step <= i1 ? i + j * step : i;
+        const int64_t at = part_at(a, hk, tile, p, p == i0 ? end0 : 0) + rr;
+        m[j] = a.part_ml[2 * at];
+        l[j] = i + j * step <= i1 ? a.part_ml[2 * at + 1] : 0.0f;
+        x[j] = *reinterpret_cast<const f32x4*>(a.part_acc + at * D + d);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = l[j] == 0.0f ? 0.0f : fast_exp2(m[j] - M);
+        if (l[j] != 0.0f) v += f * x[j];             // (else the part's keys are none of this row's)
+        L += f * l[j];
+      }
     }
     if (share) {
       acc_s[tid] = v;
