@@ -29,7 +29,8 @@
 // list for each KV head and tile of query rows, and each block takes an equal part of
 // it: with lengths that differ 8-fold no block is longer than another.  A part that
 // starts or ends inside a row leaves the row's sums in the workspace, at most two such
-// per part, and paged_mfma_join_kernel adds them up.  parts = 0: a block takes a whole row.
+// per part, and paged_mfma_join_kernel adds them up.  Where no row is much longer than a
+// part, or with parts = 0, a block takes a whole row instead.
 //
 // A load covers whole 128-byte lines where a key is one or more (a pair of loads takes
 // half-lines of its own rows and of rows 8 away, and the lanes exchange them), and is
@@ -131,13 +132,13 @@ struct PagedV {
   float scale;
 };
 
-#ifndef V_AHEAD
-#define V_AHEAD (!E8 && R == 1 && D == 128)
-#endif
-// Whether K of the next step is loaded ahead (where the registers hold it).
+// Whether K of the next step is loaded ahead: 16-bit pages at head_dim 128 (128 K keys 104 us,
+// 112 without; 16 ragged rows 63.5 and 64.6).  8-bit pages need the registers for their
+// conversions (64 rows of drafts 131 us ahead, 124 without), and at head_dim 64 a third
+// wave a SIMD hides more (64 rows of 4096 keys 42.5 us ahead, 39.4 without).
 template <bool E8, int D, int R>
 struct PagedAhead {
-  static constexpr bool value = V_AHEAD;
+  static constexpr bool value = !E8 && R == 1 && D == 128;
 };
 
 template <typename T, bool E8, int D, int R, bool STREAM>
@@ -468,6 +469,7 @@ struct UnitList {
   int b0;                    // first row held
   int units, end;            // the lane's row: its units, and the list's up to it
   int before;                // units of the rows before b0
+  int longest;               // most units of a row (after total())
 
   __device__ inline int vis_of(const RowKeys& rk) const {
     // the last query token that is real (tokens behind query_lens see nothing)
@@ -489,12 +491,20 @@ struct UnitList {
   __device__ inline int held_end() const { return __builtin_amdgcn_readlane(end, 63); }
   // the whole list's units; rows [0, 64) are held afterwards
   __device__ inline int total() {
-    int t = 0;
+    int t = 0, most = 0;
     for (int b = (a->B - 1) / 64 * 64; b > 0; b -= 64) {
       hold(b, 0);
       t += held_end();
+      most = units > most ? units : most;
     }
     hold(0, 0);
+    most = units > most ? units : most;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) {
+      const int x = __shfl_xor(most, i, 64);
+      most = x > most ? x : most;
+    }
+    longest = __builtin_amdgcn_readfirstlane(most);
     return t + held_end();
   }
 };
@@ -511,6 +521,10 @@ struct Parts {
     q = used > 0 ? total / used : 0;
     more = total - q * used;
   }
+  // Whether a block takes a row instead: no row is much longer than a part, so dividing
+  // them would only cost the joins (256 rows of up to 1024 keys, head_dim 64: 37 us by row,
+  // 53 in parts; 64 rows of up to 8192, head_dim 128: 134 and 124).
+  __device__ inline bool by_row(int longest) const { return longest <= q + (q >> 2) + 8; }
   __device__ inline int start(int i) const { return i * q + (i < more ? i : more); }
   // the part that holds unit x
   __device__ inline int of(int x) const {
@@ -564,12 +578,15 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
 
   // this block's units [u, u1) and the row b that they start in, whose units start at row_u
   int b = part, u = 0, u1 = 0, row_u = 0;
+  bool by_row = a.parts == 0;
   if (a.parts > 0) {
-    const int total = list.total();
-    const Parts parts(total, a.parts);
-    if (part >= parts.used) return;
+    const Parts parts(list.total(), a.parts);
+    by_row = parts.by_row(list.longest);
+    if (part >= (by_row ? a.B : parts.used)) return;
     u = parts.start(part);
     u1 = parts.start(part + 1);
+  }
+  if (!by_row) {
     while (list.held_end() <= u) list.hold(list.b0 + 64, list.held_end());
     const int at = (int)__builtin_ctzll(__ballot(list.end > u));
     b = list.b0 + at;
@@ -598,7 +615,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
     int hi = vis;
     bool whole = true;       // this block has all of the row's keys
     w.lo = 0;
-    if (a.parts > 0) {
+    if (!by_row) {
       const int from = u - row_u, to = u1 - row_u < units ? u1 - row_u : units;
       whole = from == 0 && to == units;
       w.lo = from * 64;
@@ -730,7 +747,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
       }
     }
     // the next row with keys
-    if (a.parts == 0) break;
+    if (by_row) break;
     u = row_u + units;
     if (u >= u1) break;
     __syncthreads();                               // LDS is written again
@@ -762,13 +779,13 @@ __global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
   list.lane = lane;
   list.s_first = row0 / a.group;
   list.s_last = (row0 + rows - 1) / a.group;
-  const int total = list.total();
+  const Parts parts(list.total(), a.parts);
+  if (parts.by_row(list.longest)) return;          // every row is written, the empty ones too
   while (list.b0 + 64 <= b) list.hold(list.b0 + 64, list.held_end());
   const int end = __builtin_amdgcn_readlane(list.end, b - list.b0);
   const int units = __builtin_amdgcn_readlane(list.units, b - list.b0);
   const int first_u = end - units;
   const int grp = tid / (D / 4), d = 4 * (tid % (D / 4));
-  const Parts parts(total, a.parts);
   int i0 = 0, i1 = -1, end0 = 0;
   if (units > 0) {
     i0 = parts.of(first_u);

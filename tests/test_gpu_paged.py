@@ -310,6 +310,43 @@ def test_attend_matches_oracle(dev, case, splits):
                  num_splits=splits)
 
 
+# rows long enough to be divided: several parts a row, parts of several rows, empty rows
+LONG = [
+    (BF16, "e4m3", 4, 2, 64, 64, 1, [2100, 70, 0, 1300], None),
+    (F16, "e4m3", 3, 1, 128, 16, 2, [65, 0, 1900, 3], [2, 0, 2, 1]),
+    (BF16, "same", 4, 2, 128, 32, 1, [1, 1601, 64], None),
+    (F16, "same", 2, 2, 64, 128, 4, [1500, 1024], None),
+    (BF16, "e4m3", 2, 2, 256, 256, 1, [700, 1], None),
+    (BF16, "e4m3", 20, 1, 64, 64, 2, [900, 1, 1200], None),
+    (F16, "same", 10, 1, 128, 64, 5, [1100, 30], [5, 3]),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(str(x) for x in c[:7]))
+@pytest.mark.parametrize("splits", [None, 2, 5, 9, 64])
+def test_attend_divided_rows_match_oracle(dev, case, splits):
+    dtype, store, Hq, Hkv, D, P, S, lens, qlens = case
+    B, slots = len(lens), (max(lens) + P - 1) // P
+    n = B * slots + 1
+    k, v, sc = make_pages(n, Hkv, P, D, dtype, store, 75)
+    table = table_of(B, slots, n, 76)
+    _dirty(k, v, sc, table, lens, P)
+    check_attend(dev, randn((B, Hq, S, D), 77, dtype), k, v, sc, table, lens, qlens, dtype=dtype,
+                 num_splits=splits)
+
+
+def test_attend_one_long_row_among_many(dev):
+    """140 rows, three of them long, around the ends of its 64s: the list of keys is held 64
+    rows at a time."""
+    B, P, slots = 140, 64, 40
+    k, v, sc = make_pages(100, 1, P, 64, F16, "e4m3", 78)
+    table = torch.randint(0, 100, (B, slots), generator=torch.Generator().manual_seed(79)).int()
+    lens = [(7 * i) % 90 for i in range(B)]
+    lens[64], lens[127], lens[139] = 2500, 2300, 2048
+    for splits in (None, 6, 200):
+        check_attend(dev, randn((B, 2, 1, 64), 74, F16), k, v, sc, table, lens, dtype=F16, num_splits=splits)
+
+
 def _dirty(k, v, sc, table, lens, P):
     """NaN behind every row's keys and in pages that are nobody's."""
     used = set()
@@ -345,12 +382,12 @@ def test_attend_reads_no_key_behind_the_last(dev, store, dtype, D, S):
 
 @pytest.mark.parametrize("store", ["same", "e4m3"])
 @pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (BF16, 128), (F32, 32)])
-@pytest.mark.parametrize("S,lens", [(5, [70, 66]), (40, [64, 90])])
+@pytest.mark.parametrize("S,lens", [(5, [70, 66]), (40, [64, 90]), (5, [1470, 1026])])
 def test_attend_a_nan_reaches_only_tokens_that_see_it(dev, store, dtype, D, S, lens):
     """A NaN value at a newer token's position: the tokens before it stay finite, those from
     it on are NaN; a NaN in K likewise."""
     P, B = 32, 2
-    slots = 3
+    slots = (max(lens) + P - 1) // P
     k, v, sc = make_pages(B * slots, 2, P, D, dtype, store, 90)
     table = table_of(B, slots, B * slots, 91)
     for b, (back, what) in enumerate(((2, "v"), (3, "k"))):
@@ -545,12 +582,38 @@ def test_captured_step_follows_its_inputs(dev, dtype, store):
         assert torch.equal(bits(cache.k), bits(twin.k)) and torch.equal(bits(cache.v), bits(twin.v))
 
 
+def test_captured_attention_of_divided_rows(dev):
+    """Two graphs over rows whose lengths move between empty, short and long: divided or
+    by row, whichever the lengths of the replay call for."""
+    from src.paged import paged_flash_attention
+    B, P, D, slots = 3, 64, 64, 40
+    cache = cache_of(dev, *make_pages(B * slots, 2, P, D, BF16, "e4m3", 170), BF16)
+    table = table_of(B, slots, B * slots, 171).to(dev)
+    q = randn((B, 4, 1, D), 172, device=dev)
+    lens = torch.full((B,), 100, dtype=torch.int64, device=dev)
+    call = (lambda: paged_flash_attention(q, cache, 0, table, lens, return_lse=True))
+    call()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    for i, now in enumerate(([2500, 3, 0], [0, 0, 0], [900, 900, 900], [1, 2560, 2559], [64, 65, 63])):
+        lens.copy_(torch.tensor(now))
+        q.copy_(randn(q.shape, 173 + i))
+        graphs[i % 2].replay()
+        ref = call()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i % 2][0], ref[0]) and torch.equal(outs[i % 2][1], ref[1]), now
+
+
 def test_calls_on_two_streams_at_once(dev):
     from src.paged import paged_flash_attention
-    P, D, lens = 64, 128, [1000, 777]
-    k, v, sc = make_pages(40, 2, P, D, BF16, "e4m3", 160)
+    P, D, lens = 64, 128, [3000, 777]
+    k, v, sc = make_pages(100, 2, P, D, BF16, "e4m3", 160)
     cache = cache_of(dev, k, v, sc, BF16)
-    table = table_of(2, 16, 40, 161).to(dev)
+    table = table_of(2, 48, 100, 161).to(dev)
     sl = torch.tensor(lens, device=dev)
     qs = [randn((2, 8, 1, D), 162 + i, device=dev) for i in range(2)]
     ref = [paged_flash_attention(q, cache, 0, table, sl) for q in qs]
