@@ -1,14 +1,17 @@
-// Attention of the newest tokens over a paged KV cache: host side, the kernel for
-// every type and head_dim, and the join of split keys.
+// Attention of the newest tokens over a paged KV cache: host side, the kernel for the
+// head_dims that are not 64, 128 or 256, and its join of split keys.
 //
 // out[b, h, s] = sum_j softmax_j(scale * q[b, h, s] . k[j]) v[j] over the keys
 // j < seq_lens[b] - n_b + s + 1 of row b (n_b query tokens, the newest of its
 // keys); 0 for a row that sees none.
 //
-// paged_attn_kernel (below) computes it in fp32 for any type and head_dim up to
-// 256, one block for each (row, head, token, key range), a wave taking 64 keys at a
-// time: the lane's key against q from LDS, the softmax across the wave, then a lane
-// per dim over the transposed V.  bf16 and fp16 at head_dim 64, 128 and 256 run on the matrix cores instead (paged_attn_mfma.hpp).
+// head_dim 64, 128 and 256 run on the matrix cores (paged_attn_mfma.hpp).  For the others
+// up to 256 paged_attn_kernel (below) computes it in fp32, one block for each (row, head,
+// token, key range), a wave taking 64 keys at a time: the lane's key against q from LDS,
+// the softmax across the wave, then a lane per dim over the transposed V.  Bound by its
+// scalar products: a block has one query row, so each of the group's rows reads the keys
+// again (8 rows of 2048 fp32 keys, 32 heads over 8 of 128, took 62.7 us on it and take
+// 33.9 on the matrix cores).
 #include <initializer_list>
 
 #include "paged_attn_kernels.hpp"
@@ -239,8 +242,8 @@ int32_t launch_attn(const PagedAttnArgs& a, bool e8, hipStream_t st) {
 
 using namespace mi;
 
-// num_splits counts parts of a KV head's keys over all rows; the kernel of any type divides
-// each row's keys alike.
+// num_splits counts parts of a KV head's keys over all rows; paged_attn_kernel divides each
+// row's keys alike.
 static int64_t ranges_per_row(int64_t num_splits, int64_t batch) {
   const int64_t n = num_splits / batch;
   return n < 1 ? 1 : (n > 256 ? 256 : n);
@@ -350,7 +353,7 @@ extern "C" int32_t mi_paged_attn(
     return ok;
   };
   a.q_vec = rows_of(q, 16, {q_sb, q_sh, q_ss});
-  a.o_vec = rows_of(out, 8, {o_sb, o_sh, o_ss});
+  a.o_vec = rows_of(out, 4 * es, {o_sb, o_sh, o_ss});
   hipStream_t st = (hipStream_t)stream;
   int32_t rc = MI_OK;
   if (plan.mfma)

@@ -24,7 +24,7 @@ struct PagedAttnArgs {
   int32_t B, Hq, Hkv, group, S, D, P, p_shift, slots, splits;
   int32_t tiles, parts, kv_rows;   // matrix cores: see PagedPlan; query rows of a block
   float scale_log2;
-  int32_t q_vec, o_vec;     // q rows 16-byte, out rows 8-byte aligned
+  int32_t q_vec, o_vec;     // q rows 16-byte, 4 elements of out rows aligned
 };
 
 // How a call is laid on blocks.

@@ -6,13 +6,13 @@ namespace mi {
 PagedPlan paged_plan(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t seq_len,
                      int64_t head_dim, int32_t dtype, int64_t num_splits) {
   PagedPlan p{};
-  p.mfma = dtype != MI_DTYPE_F32 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
+  p.mfma = head_dim == 64 || head_dim == 128 || head_dim == 256;
   if (!p.mfma) return p;
   const int64_t n = seq_len * (n_heads / n_kv_heads);
   // 2 tiles a block where one does not hold all rows and the registers hold two: each key
   // is read and widened half as often (511 tokens over 4096 keys, head_dim 64: 47 us, 54 with
   // one tile and 53 with four, whose registers leave one wave a SIMD)
-  p.r = n <= 16 || head_dim > 128 ? 1 : 2;
+  p.r = n <= 16 || head_dim > (dtype == MI_DTYPE_F32 ? 64 : 128) ? 1 : 2;
   p.tiles = (n + 16 * p.r - 1) / (16 * p.r);
   p.parts = num_splits <= 1 ? 0 : num_splits;
   return p;
@@ -56,11 +56,19 @@ void launch_tiles(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
 }
 
 template <typename T, bool E8>
+void launch_128(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.r == 2) return launch_tiles<T, E8, 128, 2>(a, p, st);
+  }
+  launch_tiles<T, E8, 128, 1>(a, p, st);
+}
+
+template <typename T, bool E8>
 void launch(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
   if (a.D == 64)
     p.r == 1 ? launch_tiles<T, E8, 64, 1>(a, p, st) : launch_tiles<T, E8, 64, 2>(a, p, st);
   else if (a.D == 128)
-    p.r == 1 ? launch_tiles<T, E8, 128, 1>(a, p, st) : launch_tiles<T, E8, 128, 2>(a, p, st);
+    launch_128<T, E8>(a, p, st);
   else
     launch_tiles<T, E8, 256, 1>(a, p, st);
 }
@@ -71,6 +79,8 @@ void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32
                             hipStream_t st) {
   if (dtype == MI_DTYPE_BF16)
     e8 ? launch<bf16_t, true>(a, plan, st) : launch<bf16_t, false>(a, plan, st);
+  else if (dtype == MI_DTYPE_F32)
+    e8 ? launch<float, true>(a, plan, st) : launch<float, false>(a, plan, st);
   else
     e8 ? launch<f16_t, true>(a, plan, st) : launch<f16_t, false>(a, plan, st);
 }

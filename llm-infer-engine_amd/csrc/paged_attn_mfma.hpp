@@ -1,5 +1,5 @@
-// Attention over a paged KV cache on the matrix cores: bf16 / fp16 queries, pages of
-// the same type or of 8-bit floats, head_dims that are multiples of 64.
+// Attention over a paged KV cache on the matrix cores: pages of the queries' type or of
+// 8-bit floats, head_dim 64, 128 and 256.
 //
 // A wave holds R tiles of 16 query rows of one KV head (row = token * group + head of
 // the group) and streams its keys from memory straight into matrix operands: nothing
@@ -10,7 +10,7 @@
 //                    pieces of its key.
 //   softmax          the accumulator gives lane (g, r) = (lane / 16, lane % 16) four
 //                    keys of row r per tile.  Which key is which row of A is free too:
-//                    tile t's row 4g + i is key g * CK + 4t + i (CK = 16 or 8), so
+//                    tile t's row 4g + i is key g * CK + 4t + i (CK = 16, 8 or 4), so
 //                    that lane (g, r) ends up with the CK neighbouring keys g * CK ..
 //                    of row r, and the row's largest score is two lane swaps away.
 //   O^T += V^T P^T   A = 16 dims x 32 keys, B = 32 keys x 16 rows.  P^T's lane (g, r)
@@ -21,7 +21,8 @@
 // V's page scale is the instruction's scale operand (bf16 has fp32's range, so no page
 // overflows), K's multiplies the scores.  p goes in as a 16-bit value and its remainder
 // (two products): off by 2^-16 at most, where one rounding of p to q's type would add an
-// error as large as that of the output itself.  l sums p in fp32.
+// error as large as that of the output itself.  l sums p in fp32.  fp32 queries run on
+// v_mfma_f32_16x16x4 in the same layout, 4 dims (keys) a lane, and p as it is.
 //
 // The block's 4 waves take every 4th step of its keys and join through LDS at the end.
 //
@@ -86,6 +87,24 @@ template <> struct MatOp<f16_t> {
   }
 };
 
+// fp32 operands are 4 dims (or keys) a lane, multiplied with v_mfma_f32_16x16x4 one by one
+template <> struct MatOp<float> {
+  typedef f32x4 v8;
+  static __device__ inline f32x4 mul(v8 a, v8 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// 4 8-bit entries (a dword) as an fp32 operand
+__device__ inline f32x4 widen4(uint32_t x, float scale) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, scale, false);
+  const f2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x, scale, true);
+  return f32x4{a[0], a[1], b[0], b[1]};
+}
+
 // 8 entries (two dwords of 8-bit values) as a matrix operand
 template <typename T>
 __device__ inline typename MatOp<T>::v8 widen8(uint32_t a, uint32_t b, float scale) {
@@ -108,14 +127,17 @@ __device__ inline float swap32(float x, int lane) {
 
 template <typename T, bool E8, int D>
 struct PagedGeom {
-  static constexpr int CK = E8 ? 16 : 8;          // neighbouring keys of a lane
+  static constexpr bool F32 = std::is_same<T, float>::value;
+  static constexpr int ES = E8 ? 1 : (int)sizeof(T);
+  static constexpr int CK = 16 / ES;              // neighbouring keys of a lane
   static constexpr int STEP = 4 * CK;             // keys of a step
   static constexpr int KT = CK / 4;               // 16-key tiles of a step
-  static constexpr int KL = E8 ? D / 64 : D / 32; // 16-byte loads of a key by a lane
+  static constexpr int KL = D * ES / 64;          // 16-byte loads of a key by a lane
   static constexpr bool PAIRS = KL % 2 == 0;      // a key is whole 128-byte lines
   static constexpr int VL = D / 16;               // 16-byte loads of V by a lane
-  static constexpr int U = CK / 8;                // P.V products' key groups of 32
-  static constexpr int ES = E8 ? 1 : 2;
+  static constexpr int OE = F32 ? 4 : 8;          // dims (keys) of an operand that a lane holds
+  static constexpr int NJ = D / (4 * OE);         // Q.K operands of a tile
+  static constexpr int U = CK / OE;               // P.V operands of a step
 };
 
 // One step's keys and values, as loaded.
@@ -136,9 +158,9 @@ struct PagedV {
 // 112 without; 16 ragged rows 63.5 and 64.6).  8-bit pages need the registers for their
 // conversions (64 rows of drafts 131 us ahead, 124 without), and at head_dim 64 a third
 // wave a SIMD hides more (64 rows of 4096 keys 42.5 us ahead, 39.4 without).
-template <bool E8, int D, int R>
+template <typename T, bool E8, int D, int R>
 struct PagedAhead {
-  static constexpr bool value = !E8 && R == 1 && D == 128;
+  static constexpr bool value = sizeof(T) == 2 && !E8 && R == 1 && D == 128;
 };
 
 template <typename T, bool E8, int D, int R, bool STREAM>
@@ -146,7 +168,7 @@ struct PagedWave {
   typedef PagedGeom<T, E8, D> G;
   typedef PagedK<T, E8, D> KStep;
   typedef PagedV<T, E8, D> VStep;
-  typedef typename std::conditional<E8, bf16_t, T>::type PT;   // what P and V multiply in
+  typedef typename std::conditional<E8 && !G::F32, bf16_t, T>::type PT;   // what P and V multiply in
   typedef typename MatOp<T>::v8 Q8;
   typedef typename MatOp<PT>::v8 P8;
 
@@ -161,7 +183,7 @@ struct PagedWave {
   int lo, lim, minvis;        // keys [lo, lim); all rows that see any of them see [lo, minvis)
   bool v_once;                // a step takes whole lines of V
   float scale_log2;
-  Q8 q[R][D / 32];
+  Q8 q[R][G::NJ];
   f32x4 o[R][D / 16];
   float m[R], l[R];
   int vis[R];
@@ -257,9 +279,17 @@ struct PagedWave {
               from_other_half<0x3>(y.z, x.z), from_other_half<0x3>(y.w, x.w)};
   }
 
-  // K operand j (32 dims) of tile t
+  // the first dim of this lane in K operand j
+  __device__ inline int dim_of(int j) const {
+    if constexpr (!E8) return (j * 4 + g) * G::OE;
+    constexpr int per = 16 / G::OE;                // operands of a 16-byte piece
+    return j / per * 64 + g * 16 + j % per * G::OE;
+  }
+  // K operand j of tile t
   __device__ inline Q8 k_op(const KStep& st, int t, int j) const {
-    if constexpr (E8) {
+    if constexpr (E8 && G::F32) {
+      return widen4(st.k[t][j >> 2][j & 3], 1.0f);
+    } else if constexpr (E8) {
       const u32x4 w = st.k[t][j >> 1];
       return (j & 1) ? widen8<T>(w.z, w.w, 1.0f) : widen8<T>(w.x, w.y, 1.0f);
     } else {
@@ -267,11 +297,15 @@ struct PagedWave {
     }
   }
   // V operand u of dims 16 i .. 16 i + 15
-  __device__ inline P8 v_op(const u32x4& v, int u, float vs) const {
-    if constexpr (E8)
-      return u == 0 ? widen8<PT>(v.x, v.y, vs) : widen8<PT>(v.z, v.w, vs);
-    else
-      return __builtin_bit_cast(P8, v);
+  __device__ inline P8 v_op(const VStep& st, int i, int u) const {
+    if constexpr (E8 && G::F32) {
+      return widen4(st.v[i][u], st.scale);
+    } else if constexpr (E8) {
+      const u32x4 v = st.v[i];
+      return u == 0 ? widen8<PT>(v.x, v.y, st.scale) : widen8<PT>(v.z, v.w, st.scale);
+    } else {
+      return __builtin_bit_cast(P8, st.v[i]);
+    }
   }
   // v with the keys outside [a, b) of the lane's CK zeroed
   __device__ inline u32x4 keep(const u32x4& v, int a, int b) const {
@@ -292,6 +326,8 @@ struct PagedWave {
     constexpr bool bf = std::is_same<T, bf16_t>::value;
     if constexpr (E8)
       return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    else if constexpr (G::F32)
+      return ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
     else
       return ((w & (bf ? 0x7f807f80u : 0x7c007c00u)) + (bf ? 0x00800080u : 0x04000400u)) & 0x80008000u;
   }
@@ -299,10 +335,10 @@ struct PagedWave {
     return (not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w)) != 0;
   }
   __device__ inline uint32_t finite_part(uint32_t w) const {
-    return w & ~((not_finite(w) >> (8 * G::ES - 1)) * (E8 ? 0xffu : 0xffffu));
+    return w & ~((not_finite(w) >> (8 * G::ES - 1)) * (E8 ? 0xffu : G::F32 ? 0xffffffffu : 0xffffu));
   }
 
-  P8 hi[R][G::U], rest[R][G::U];   // p of the step: its 16-bit value and the remainder
+  P8 hi[R][G::U], rest[R][G::U];   // p of the step: its 16-bit value and the remainder (fp32: hi)
   bool whole, here;                // the step's keys are all seen by all rows; `live`
 
   // scores, softmax and p of the step at `base`
@@ -311,25 +347,28 @@ struct PagedWave {
     here = live(base, pg);
     f32x4 s[R][G::KT];
     // two tiles at a time: products into one accumulator wait for each other
+    constexpr int kTiles = G::KT < 2 ? G::KT : 2;
 #pragma unroll
-    for (int t = 0; t < G::KT; t += 2) {
+    for (int t0 = 0; t0 < G::KT; t0 += kTiles) {
       if constexpr (G::PAIRS) {
 #pragma unroll
-        for (int i = 0; i < G::KL; i += 2) {
-          exchange(st.k[t][i], st.k[t][i + 1]);
-          exchange(st.k[t + 1][i], st.k[t + 1][i + 1]);
-        }
+        for (int i = 0; i < G::KL; i += 2)
+#pragma unroll
+          for (int t = t0; t < t0 + kTiles; ++t) exchange(st.k[t][i], st.k[t][i + 1]);
       }
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) s[rt][t] = s[rt][t + 1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int rt = 0; rt < R; ++rt)
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const Q8 a0 = k_op(st, t, j), a1 = k_op(st, t + 1, j);
+        for (int t = t0; t < t0 + kTiles; ++t) s[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int rt = 0; rt < R; ++rt) {
-          s[rt][t] = MatOp<T>::mul(a0, q[rt][j], s[rt][t]);
-          s[rt][t + 1] = MatOp<T>::mul(a1, q[rt][j], s[rt][t + 1]);
-        }
+      for (int j = 0; j < G::NJ; ++j) {
+        Q8 k[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) k[t] = k_op(st, t0 + t, j);
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) s[rt][t0 + t] = MatOp<T>::mul(k[t], q[rt][j], s[rt][t0 + t]);
       }
     }
     // (not below the least normal number: -inf times it must stay -inf)
@@ -365,19 +404,27 @@ struct PagedWave {
       float sum = 0.0f;
 #pragma unroll
       for (int u = 0; u < G::U; ++u) {
-        uint32_t h[4], x[4];
+        if constexpr (G::F32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 8 * u + 2 * e;
-          const float p0 = fast_exp2(fmaf(s[rt][k >> 2][k & 3], c, -m_new));
-          const float p1 = fast_exp2(fmaf(s[rt][k >> 2][(k & 3) + 1], c, -m_new));
-          sum += p0 + p1;
-          float h0, h1;
-          h[e] = MatOp<PT>::pack(p0, p1, h0, h1);
-          x[e] = MatOp<PT>::pack(p0 - h0, p1 - h1, h0, h1);
+          for (int e = 0; e < 4; ++e) {
+            hi[rt][u][e] = fast_exp2(fmaf(s[rt][u][e], c, -m_new));
+            sum += hi[rt][u][e];
+          }
+        } else {
+          uint32_t h[4], x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 8 * u + 2 * e;
+            const float p0 = fast_exp2(fmaf(s[rt][k >> 2][k & 3], c, -m_new));
+            const float p1 = fast_exp2(fmaf(s[rt][k >> 2][(k & 3) + 1], c, -m_new));
+            sum += p0 + p1;
+            float h0, h1;
+            h[e] = MatOp<PT>::pack(p0, p1, h0, h1);
+            x[e] = MatOp<PT>::pack(p0 - h0, p1 - h1, h0, h1);
+          }
+          hi[rt][u] = __builtin_bit_cast(P8, u32x4{h[0], h[1], h[2], h[3]});
+          rest[rt][u] = __builtin_bit_cast(P8, u32x4{x[0], x[1], x[2], x[3]});
         }
-        hi[rt][u] = __builtin_bit_cast(P8, u32x4{h[0], h[1], h[2], h[3]});
-        rest[rt][u] = __builtin_bit_cast(P8, u32x4{x[0], x[1], x[2], x[3]});
       }
       l[rt] = l[rt] * alpha + sum;
     }
@@ -413,16 +460,18 @@ struct PagedWave {
       for (int u = 0; u < G::U; ++u) {
         P8 a[kTogether];
 #pragma unroll
-        for (int j = 0; j < kTogether; ++j) a[j] = v_op(st.v[i + j], u, st.scale);
+        for (int j = 0; j < kTogether; ++j) a[j] = v_op(st, i + j, u);
 #pragma unroll
         for (int rt = 0; rt < R; ++rt) {
 #pragma unroll
           for (int j = 0; j < kTogether; ++j) o[rt][i + j] = MatOp<PT>::mul(a[j], hi[rt][u], o[rt][i + j]);
         }
+        if constexpr (!G::F32) {
 #pragma unroll
-        for (int rt = 0; rt < R; ++rt) {
+          for (int rt = 0; rt < R; ++rt) {
 #pragma unroll
-          for (int j = 0; j < kTogether; ++j) o[rt][i + j] = MatOp<PT>::mul(a[j], rest[rt][u], o[rt][i + j]);
+            for (int j = 0; j < kTogether; ++j) o[rt][i + j] = MatOp<PT>::mul(a[j], rest[rt][u], o[rt][i + j]);
+          }
         }
       }
     }
@@ -642,9 +691,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
       const T* qp =
           static_cast<const T*>(a.q) + b * a.q_sb + (hk * a.group + hg) * a.q_sh + s * a.q_ss;
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        // the dims of K's operand j
-        const int d = E8 ? (j >> 1) * 64 + w.g * 16 + (j & 1) * 8 : j * 32 + w.g * 8;
+      for (int j = 0; j < G::NJ; ++j) {
+        const int d = w.dim_of(j);
         typename Wave::Q8 x;
         if (!real) {
           x = __builtin_bit_cast(typename Wave::Q8, u32x4{0u, 0u, 0u, 0u});
@@ -652,7 +700,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
           x = __builtin_bit_cast(typename Wave::Q8, load16(qp + d));
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = qp[d + e];
+          for (int e = 0; e < G::OE; ++e) x[e] = qp[d + e];
         }
         w.q[rt][j] = x;
       }
@@ -660,7 +708,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
 
     if (base < hi) {
       typename Wave::VStep v;
-      if constexpr (PagedAhead<E8, D, R>::value) {
+      if constexpr (PagedAhead<T, E8, D, R>::value) {
         // K of the next step is on its way from before this step's products, V of the next
         // from behind them
         typename Wave::KStep ka, kb;

@@ -294,6 +294,13 @@ ATTEND = [
     (BF16, "e4m3", 4, 2, 80, 16, 3, [50, 3], None),
     (F32, "same", 4, 2, 64, 16, 3, [50, 97], None),
     (F32, "e4m3", 4, 2, 6, 32, 2, [50, 97], [1, 2]),
+    (F32, "same", 4, 2, 32, 64, 1, [65, 1], None),
+    (F32, "e4m3", 4, 2, 64, 64, 11, [50, 97], [11, 2]),
+    (F32, "same", 8, 2, 128, 32, 1, [1, 17, 64, 200, 0], None),
+    (F32, "e4m3", 6, 2, 128, 16, 4, [4, 129, 300], [4, 3, 0]),
+    (F32, "same", 4, 2, 256, 64, 5, [77, 64], None),
+    (F32, "e4m3", 16, 1, 256, 256, 2, [77, 300], None),
+    (F32, "same", 4, 1, 64, 16, 70, [100, 70], None),
 ]
 
 
@@ -319,6 +326,11 @@ LONG = [
     (BF16, "e4m3", 2, 2, 256, 256, 1, [700, 1], None),
     (BF16, "e4m3", 20, 1, 64, 64, 2, [900, 1, 1200], None),
     (F16, "same", 10, 1, 128, 64, 5, [1100, 30], [5, 3]),
+    (F32, "same", 4, 2, 128, 16, 1, [1600, 1, 0, 700], None),
+    (F32, "e4m3", 20, 1, 64, 64, 2, [900, 1, 1200], None),
+    (F32, "same", 2, 2, 64, 256, 3, [1200, 1030], [3, 1]),
+    (F32, "e4m3", 2, 1, 256, 32, 1, [1500], None),
+    (F32, "same", 3, 3, 48, 16, 1, [1100, 0, 300], None),
 ]
 
 
@@ -366,7 +378,7 @@ def _dirty(k, v, sc, table, lens, P):
 
 
 @pytest.mark.parametrize("store", ["same", "e4m3"])
-@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 32)])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (F32, 32), (F32, 64), (F32, 128)])
 @pytest.mark.parametrize("S", [1, 3])
 def test_attend_reads_no_key_behind_the_last(dev, store, dtype, D, S):
     P, lens = 16, [1, 15, 16, 49, 100, 0]
@@ -381,7 +393,7 @@ def test_attend_reads_no_key_behind_the_last(dev, store, dtype, D, S):
 
 
 @pytest.mark.parametrize("store", ["same", "e4m3"])
-@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (BF16, 128), (F32, 32)])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 128), (BF16, 128), (F32, 32), (F32, 128)])
 @pytest.mark.parametrize("S,lens", [(5, [70, 66]), (40, [64, 90]), (5, [1470, 1026])])
 def test_attend_a_nan_reaches_only_tokens_that_see_it(dev, store, dtype, D, S, lens):
     """A NaN value at a newer token's position: the tokens before it stay finite, those from
@@ -405,7 +417,7 @@ def test_attend_a_nan_reaches_only_tokens_that_see_it(dev, store, dtype, D, S, l
 
 
 @pytest.mark.parametrize("store", ["same", "e4m3"])
-@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F32, 64)])
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F32, 64), (F32, 40)])
 def test_attend_skips_entries_that_are_no_page(dev, store, dtype, D):
     P, lens = 16, [80, 80, 10 ** 12, -5, 64]
     B, slots = len(lens), 5
