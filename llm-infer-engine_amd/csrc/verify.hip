@@ -57,38 +57,33 @@ struct VerifyArgs {
   int32_t B, S, rows, chunks, greedy;
 };
 
-// Shares 2^((x - m) c) of logits x <= m.  y = (x - m) c in fp64; y = k / 32 + f, |f| <=
-// 1/64, k from the low bits of y + 1.5 * 2^47; 2^(k/32) is a table entry with k / 32's whole
-// part added to its exponent, 2^f = 1 + f p(f) with p the series of ln 2 (f ln 2)^i / (i+1)!
-// in fp32, off by 2^-24 of 0.011.  The table's 32 doubles lie on all 64 LDS banks once: no
-// lanes collide.
+// Shares 2^((x - m) c) of logits x <= m.  y = (x - m) c in fp64, held to [-1100, 0] (a NaN or
+// -inf is then 0 in the end, +inf the largest); y = k / 32 + f, |f| <= 1/64, k from the low
+// bits of y + 1.5 * 2^47; 2^(k/32) is a table entry times 2^(k/32's whole part), 2^f =
+// 1 + f p(f) with p the series of ln 2 (f ln 2)^i / (i+1)! in fp32, off by 2^-24 of 0.011.
+// The table's 32 doubles lie on all 64 LDS banks once: no lanes collide.
 struct Shares {
   const double* table;      // LDS: 2^(i/32)
-  double c, mc;             // scale, m * scale
-  float m, lo;              // below lo a share is 0 (2^-1000)
+  double c, least;          // scale, the least x - m
+  float m;
   __device__ inline void set(const double* t, float top, double scale) {
     table = t;
     m = top;
     c = scale;
-    mc = (double)top * scale;
-    lo = top - (float)(1000.0 / scale);
+    least = -1100.0 / scale;
   }
   __device__ inline double of(float x) const {
-    const bool in = x >= lo;
-    const double xd = (double)(in ? x : m);
     const double magic = 211106232532992.0;         // 1.5 * 2^47
-    const double y = fma(xd, c, -mc), z = y + magic;
+    const double d = fmin(fmax((double)x - (double)m, least), 0.0), z = fma(d, c, magic);
     const int k = (int)__double_as_longlong(z);
-    const float f = (float)(y - (z - magic));
+    const float f = (float)fma(d, c, magic - z);
     float p = 0.009618129f;                           // (ln 2)^4 / 4!
     p = fmaf(p, f, 0.05550411f);                      // (ln 2)^3 / 3!
     p = fmaf(p, f, 0.24022651f);                      // (ln 2)^2 / 2!
     p = fmaf(p, f, 0.69314718f);
     p *= f;
     const double t = table[k & 31];
-    const double r = fma(t, (double)p, t);
-    const long long bits = __double_as_longlong(r) + ((long long)(k >> 5) << 52);
-    return in ? __longlong_as_double(bits) : 0.0;
+    return ldexp(fma(t, (double)p, t), k >> 5);
   }
 };
 __device__ inline void fill_table(double* t) {
@@ -112,8 +107,7 @@ __device__ inline const T* row_of(const VerifyArgs& a, int b, int row) {
 }
 
 // The thread's E logits of a chunk: groups of 16 bytes aligned in memory, dealt to
-// the threads in turn.  `first` + index is a logit's place in the row; places
-// outside the chunk's [lo, hi) hold -inf.
+// the threads in turn; places outside the chunk's [lo, hi) hold -inf.
 template <typename T, int E>
 struct ChunkLogits {
   static constexpr int N = Chunk<T>::kN;       // logits of a group
@@ -140,12 +134,10 @@ struct ChunkLogits {
       const int64_t j = place(g);
       if (aligned && j >= lo && j + N <= hi) {
         Chunk<T>::unpack(load16(row + j), x + g * N);
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[g * N + e] = logit(x[g * N + e]);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          x[g * N + e] = j + e >= lo && j + e < hi ? logit(Elem<T>::to_f32(row[j + e])) : -INFINITY;
+          x[g * N + e] = j + e >= lo && j + e < hi ? Elem<T>::to_f32(row[j + e]) : -INFINITY;
       }
     }
   }
@@ -165,7 +157,10 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   c.load(row_of<T>(a, b, row), lo, hi);
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; ++i) top = fmaxf(top, c.x[i]);
+  for (int i = 0; i < E; ++i) {
+    c.x[i] = logit(c.x[i]);
+    top = fmaxf(top, c.x[i]);
+  }
   // least place of the thread's largest logit (T = 0): its places grow with i
   int64_t at = lo;
   if (a.greedy && top > -INFINITY) {
@@ -531,8 +526,7 @@ __global__ __launch_bounds__(64) void verify_pick_kernel(VerifyArgs a) {
     x[e] = 0.0;
     if (j >= lo && j < hi) {
       double wj, pj;
-      w.get(logit(Elem<T>::to_f32(tr[j])), dr != nullptr ? logit(Elem<T>::to_f32(dr[j])) : -INFINITY, j,
-            &wj, &pj);
+      w.get(Elem<T>::to_f32(tr[j]), dr != nullptr ? Elem<T>::to_f32(dr[j]) : -INFINITY, j, &wj, &pj);
       x[e] = use_w ? wj : pj;
     }
     sum += x[e];
