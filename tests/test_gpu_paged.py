@@ -359,6 +359,23 @@ def test_attend_one_long_row_among_many(dev):
         check_attend(dev, randn((B, 2, 1, 64), 74, F16), k, v, sc, table, lens, dtype=F16, num_splits=splits)
 
 
+@pytest.mark.parametrize("dtype,store,D", [(BF16, "same", 64), (F16, "e4m3", 128), (F32, "same", 128), (F32, "same", 48)])
+@pytest.mark.parametrize("step", [0.05, 3.0, -3.0])
+def test_attend_scores_that_rise_and_fall(dev, dtype, store, D, step):
+    """Scores that grow by less than a step's worth, by much more, and that fall: the running
+    maximum moves late, in every step, and once."""
+    P, L = 16, 400
+    k, v, sc = make_pages(L // P + 1, 1, P, D, dtype, store, 126)
+    table = torch.arange(L // P + 1, dtype=torch.int32)[None]
+    at = torch.arange((L // P + 1) * P, dtype=torch.float32).view(-1, 1, P, 1) * step
+    k = (k.float() * 0.01 if store == "same" else torch.zeros(k.shape))
+    k[..., :1] += (at if store == "same" else (at / 8).clamp(-400, 400))
+    k = k.to(dtype if store == "same" else E4M3)
+    q = randn((1, 2, 3, D), 127, dtype).abs()
+    q[0, 1, 2, 0] = 0.0
+    check_attend(dev, q, k, v, sc, table, [L], dtype=dtype)
+
+
 def _dirty(k, v, sc, table, lens, P):
     """NaN behind every row's keys and in pages that are nobody's."""
     used = set()
