@@ -600,7 +600,8 @@ int32_t mi_paged_attn(
  * draft n was refused (p_n if that is zero everywhere), else w = p_n.  Temperature
  * 0: draft i is accepted iff it is the first largest logit of target[b][i], the
  * next token is that of row n, and draft, accept_u and sample_u are not read.
- * Shares and sums are fp64.  A NaN logit counts as -inf, +inf as the largest finite
+ * p and q are good to 1e-6 where they are compared; the sums that choose the token
+ * are fp64, of shares good to 1e-9.  A NaN logit counts as -inf, +inf as the largest finite
  * value; a row without mass refuses its draft and gives the token -1.  A drafted
  * token outside [0, vocab) is refused.  target [batch, drafts + 1, vocab], draft
  * [batch, drafts, vocab] (unit vocab stride), drafted and accept_u [batch, drafts],

@@ -27,6 +27,12 @@
 // runs by neighbouring threads, without LDS.  8-bit pages read their tokens twice
 // (largest value, then entries): the second read comes from the caches, and no
 // register holds a page.  Other layouts (VEC = 1) move one element at a time.
+//
+// Long prompts are bound by memory, steps by the chain of dependent reads (row's position,
+// page number, tokens, for 8-bit pages the largest value and the old scale).  Measured
+// (kernel alone): 4 x 2048 tokens of 32 + 8 + 8 heads of 64, bf16 into 8-bit pages, 92.5 MB
+// in 18.2 us, 5.1 TB/s; 1021 tokens of 128, fp16, 25.4 MB in 8.6 us; 64 rows of 4 tokens
+// into 8-bit pages 8.0 us; one token 4.1 us, an empty launch being 2 to 3.
 #include <initializer_list>
 
 #include "common.hpp"
@@ -425,7 +431,8 @@ extern "C" int32_t mi_rope_paged_append(
   // pages that seq_len tokens touch at most, wherever the first of them lies
   a.spans = (int32_t)((seq_len + page_size - 2) / page_size + 1);
   const int64_t kv_blocks = batch * a.spans * n_kv_heads;
-  // 4 waves for a page of a prompt; one wave where a block has a few tokens
+  // 4 waves for a page of a prompt; one wave where a block has a few tokens (4 x 2048 tokens
+  // 21.4 us, with one wave 25.5; 64 rows of 4 tokens 10.3 us, with 4 waves 12.1)
   const int block = seq_len > 8 ? 256 : 64;
   a.q_items = xq == nullptr ? 0 : batch * seq_len * n_heads * (head_dim / 2 / (vec ? 8 : 1));
   int64_t q_blocks = (a.q_items + block - 1) / block;

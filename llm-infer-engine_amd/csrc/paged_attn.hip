@@ -182,13 +182,15 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
   }
 }
 
-// The splits of a row joined: sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i.  A
-// wave takes one row, a lane dims lane, lane + 64, ..; it reads each partial once.
+// The splits of a row joined: sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i.  A block
+// takes a row and its waves every 4th split, a lane dims lane, lane + 64, .., four splits'
+// loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.B * a.Hq * a.S) return;
+  __shared__ float acc_s[4][256];
+  __shared__ float l_s[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
   const float* ml = a.part_ml + 2 * row * a.splits;
   const float* pa = a.part_acc + row * a.splits * a.D;
   float M = kNegBig;
@@ -196,26 +198,39 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 #pragma unroll
   for (int i = 32; i; i >>= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
   float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = 0; i < a.splits; ++i) {
-    const float l = ml[2 * i + 1];
-    if (l == 0.0f) continue;                     // an empty range has no sums
-    const float w = fast_exp2(ml[2 * i] - M);
-    L += w * l;
+  for (int i = wave; i < a.splits; i += 16) {
+    float l[4], w[4], x[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int d = lane + 64 * j;
-      if (d < a.D) o[j] += w * pa[(int64_t)i * a.D + d];
+      const bool in = i + 4 * j < a.splits;
+      const int s = in ? i + 4 * j : i;
+      l[j] = in ? ml[2 * s + 1] : 0.0f;
+      w[j] = ml[2 * s];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[j][k] = lane + 64 * k < a.D ? pa[(int64_t)s * a.D + lane + 64 * k] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (l[j] == 0.0f) continue;                // an empty range has no sums
+      const float f = fast_exp2(w[j] - M);
+      L += f * l[j];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += f * x[j][k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc_s[wave][lane + 64 * k] = o[k];
+  if (lane == 0) l_s[wave] = L;
+  __syncthreads();
+  L = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
   const int s = (int)(row % a.S);
   const int h = (int)(row / a.S % a.Hq), b = (int)(row / a.S / a.Hq);
   T* op = reinterpret_cast<T*>(a.out) + b * a.o_sb + h * a.o_sh + s * a.o_ss;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = lane + 64 * j;
-    if (d < a.D) op[d] = Elem<T>::from_f32(L == 0.0f ? 0.0f : o[j] / L);
+  if (tid < a.D) {
+    const float y = (acc_s[0][tid] + acc_s[1][tid]) + (acc_s[2][tid] + acc_s[3][tid]);
+    op[tid] = Elem<T>::from_f32(L == 0.0f ? 0.0f : y / L);
   }
-  if (lane == 0 && a.lse != nullptr)
+  if (tid == 0 && a.lse != nullptr)
     a.lse[row] = L == 0.0f ? -INFINITY : (M + fast_log2(L)) * kLn2;
 }
 
@@ -233,7 +248,7 @@ int32_t launch_attn(const PagedAttnArgs& a, bool e8, hipStream_t st) {
   else
     hipLaunchKernelGGL((paged_attn_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, a);
   if (a.splits > 1)
-    hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(paged_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, st, a);
   return MI_OK;
 }
 
@@ -260,9 +275,13 @@ extern "C" int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t 
   const PagedPlan plan = paged_plan(batch, n_heads, n_kv_heads, seq_len, head_dim, dtype, 1);
   if (plan.mfma) return paged_mfma_splits(plan, batch, n_kv_heads, head_dim, units, store);
   const int64_t blocks = batch * n_heads * seq_len;
-  // 8 blocks of 4 waves a compute unit, of 4 units of 64 keys or more each
-  int64_t s = 8 * (int64_t)device_cu_count() / blocks;
+  // 8 blocks of 4 waves a compute unit, of 4 units of 64 keys or more each; a multiple of the
+  // 8 L2s, so that the heads of a group, which read the same keys, find them in one (1 row of
+  // up to 32768 fp16 keys, 24 heads over 8 of 96: 64 splits 62 us, 85 132, 128 65; 16 rows of up
+  // to 8192, 32 over 8 of 80: 4 splits 104 us, 8 96, 16 105)
+  int64_t s = (8 * (int64_t)device_cu_count() / blocks + 7) / 8 * 8;
   if (s > (units + 3) / 4) s = (units + 3) / 4;
+  if (s > 8) s = s / 8 * 8;
   return ranges_per_row(s * batch, batch) * batch;
 }
 

@@ -35,8 +35,21 @@
 //
 // A load covers whole 128-byte lines where a key is one or more (a pair of loads takes
 // half-lines of its own rows and of rows 8 away, and the lanes exchange them), and is
-// non-temporal where no other block reads the same keys.  A row of V longer than 64 bytes
-// is taken by two waves or steps, half a line each, and stays in the caches for the second.
+// non-temporal where no other block reads the same keys (64 rows of 4 tokens, 8-bit pages: 123
+// us, 137 without; one row of 131072 bf16 keys 95 and 107).  A row of V longer than 64 bytes
+// is taken by two waves or steps, half a line each, and stays in the caches for the second
+// (16 rows, bf16, pages of 64: 64.1 us, non-temporal 64.6).
+//
+// What bounds it.  Up to 16 query rows a KV head: memory; with everything but the loads left
+// out it takes 96 to 98 % of the time.  64 rows of 4 tokens, 24 heads over 8 of 128, up to
+// 8192 8-bit keys: 614 MB in 115.6 us, 5.3 TB/s (a 4 GiB copy reaches 4.8); 16 rows of 1024 ..
+// 8192 bf16 keys in pages of 16: 317 MB in 54.2 us, 5.9 TB/s; one row of 131072 8-bit keys: 268
+// MB in 48.8 us, 5.5 TB/s.  The join of divided rows adds 5.6 to 7.8 us.  Pieces of prompts:
+// the softmax's vector instructions and the two products of p (511 tokens over 4096 8-bit
+// keys, 32 heads over 8 of 64: 43.6 us, 370 TFLOP/s of Q K and P V; without p's remainder
+// 35), and with 16-bit pages the L1, which takes the loads 16 bytes a clock, a lane a row of
+// the page (66 us).  Keys that the block's waves share in LDS are 1.1 to 1.5 times faster
+// there from 512 tokens of 4096 keys or 4 rows of 512 on, and 1.1 to 2 times slower below.
 //
 // Keys behind the last visible one: their scores are -inf and their V entries are
 // zeroed, so that nothing in them (a NaN in an old page) reaches a sum.  Where
@@ -814,7 +827,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
 // over them.  Rows without keys become 0; all others are written already.  A block takes
 // the query rows of one tile (or, where that leaves most of the GPU idle, one of
 // them), D / 4 threads a part's sums (4 dims each): with up to 4 parts the groups take
-// a query row each, else they share the parts of one.
+// a query row each, else they share the parts of one (one row of 131072 keys: 56 us in all,
+// 84 if a group took all parts).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
   constexpr int kGroups = 256 / (D / 4);

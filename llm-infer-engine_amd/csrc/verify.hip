@@ -18,7 +18,7 @@
 // sums of fp32 shares do not resolve.  Sums that choose are therefore fp64, of
 // shares good to 1e-9 of themselves (Shares below: a table of 32 powers of two and a
 // short fp32 series for what is left).  u q < p alone only compares three numbers: the
-// sums below its p and q are of fp32 shares (3e-7).
+// sums below its p and q are of fp32 shares (1e-6).
 //
 // `stats` reads every row that may matter once (chunks of 8184 or 2040 logits, each in
 // its block's registers: largest value, its index, sum of fp32 shares relative to it).
@@ -27,6 +27,12 @@
 // token.  Where w is p_n - q_n the two rows' sums have to be exact first: decide adds
 // them up, and weigh is a launch of its own; without draft logits their sum is a common
 // factor, and decide weighs itself.  T = 0 needs the first two only.
+//
+// 64 rows of 7 drafts, 128256 tokens, bf16: stats read 246 MB in 51 us, 4.8 TB/s, bound by
+// memory; decide 18.9 us and weigh 19.2, bound by their 20 vector instructions a share; pick
+// 7.9.  2 rows of 3 drafts: 4.6, 7.3, 5.3 and 6.6 us, each a launch and a chain of dependent
+// reads.  (pick as the work of a row's last block instead: the fence that shows it the
+// others' sums writes back the L2 for every block, 106 us against 97 for the 64 rows.)
 #include <algorithm>
 
 #include "common.hpp"

@@ -208,6 +208,9 @@ class Llama3(nn.Module):
             raise ValueError("page_table is required when using a PagedKVCache")
         B, S = tokens.shape
         if start_positions is None:
+            if not 0 <= int(start_pos) <= self.freqs_cis.shape[0] - S:
+                raise ValueError(f"positions {start_pos} .. {start_pos + S - 1} do not lie in "
+                                 f"[0, {self.freqs_cis.shape[0]})")
             start_positions = torch.full((B,), int(start_pos), dtype=torch.int64,
                                          device=tokens.device)
         return start_positions, start_positions + (S if query_lens is None else query_lens.clamp(0, S))

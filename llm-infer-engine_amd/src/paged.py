@@ -56,7 +56,8 @@ class PagedKVCache:
                    dtype: torch.dtype | None = None) -> "PagedKVCache":
         """A cache over existing pages (not copied): k [n_layers, num_pages, n_kv_heads,
         page_size, head_dim] or one layer's [num_pages, ..], v the same transposed, scales
-        for 8-bit pages; ``dtype`` is the activations' (default: k's)."""
+        for 8-bit pages (powers of two, as the append leaves them); ``dtype`` is the
+        activations' (default: k's)."""
         dtype = dtype if dtype is not None else k.dtype
         if k.dim() == 4:
             k, v = k[None], v[None] if v.dim() == 4 else v
@@ -119,9 +120,6 @@ def _check_pages(dtype, kv_dtype, num_pages, page_size, head_dim):
         raise ValueError(f"PagedKVCache: num_pages must be positive, got {num_pages}")
     if head_dim % 2 != 0 or not 2 <= head_dim <= 256:
         raise ValueError(f"PagedKVCache: head_dim must be even and at most 256, got {head_dim}")
-
-
-_I32, _I64 = torch.int32, torch.int64
 
 
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32

@@ -84,12 +84,12 @@ def verify_drafts(target_logits, draft_tokens, accept_u=None, sample_u=None, *,
     tokens, accepted = draft_tokens.new_empty((B, S + 1)), draft_tokens.new_empty((B,))
     if B == 0:
         return tokens, accepted
-    n = lib.mi_verify_drafts_workspace(B, S, V)
-    ws = draft_tokens.new_empty((n // 8 + 1,))
     ts, xs = target_logits.stride(), draft_tokens.stride()
     ds = (0, 0) if draft_logits is None else draft_logits.stride()
     us = (0, 0) if accept_u is None else accept_u.stride()
     with _lib.on_device(index):
+        n = lib.mi_verify_drafts_workspace(B, S, V)
+        ws = draft_tokens.new_empty((n // 8 + 1,))
         st = lib.mi_verify_drafts(
             target_logits.data_ptr(), _lib.ptr(draft_logits), draft_tokens.data_ptr(),
             _lib.ptr(accept_u), _lib.ptr(sample_u), _lib.ptr(draft_lens), tokens.data_ptr(),

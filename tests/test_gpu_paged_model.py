@@ -177,6 +177,9 @@ def test_refused_calls(dev):
     table = shuffled(1, 2, 50, dev)
     with pytest.raises(ValueError, match="page_table"):
         model(tok, kv_cache=cache)
+    for start in (-1, args.max_seq_len - 2):
+        with pytest.raises(ValueError, match="positions"):
+            model(tok, start, kv_cache=cache, page_table=table)
     with pytest.raises(ValueError, match="seq_lens"):
         model(tok, kv_cache=cache, page_table=table, seq_lens=torch.ones(1, dtype=torch.int64, device=dev))
     with pytest.raises(ValueError, match="scatter_positions"):
