@@ -28,11 +28,12 @@
 // them up, and weigh is a launch of its own; without draft logits their sum is a common
 // factor, and decide weighs itself.  T = 0 needs the first two only.
 //
-// 64 rows of 7 drafts, 128256 tokens, bf16: stats read 246 MB in 51 us, 4.8 TB/s, bound by
-// memory; decide 18.9 us and weigh 19.2, bound by their 20 vector instructions a share; pick
-// 7.9.  2 rows of 3 drafts: 4.6, 7.3, 5.3 and 6.6 us, each a launch and a chain of dependent
+// 64 rows of up to 7 drafts, 128256 tokens, bf16: stats read 214 MB in 46 us, 4.6 TB/s, bound
+// by memory (51 with each logit cleaned by itself instead of held to [-max, 0] after the
+// difference); decide 18.9 us and weigh 19.2, bound by their 20 vector instructions a share;
+// pick 7.8.  2 rows of 3 drafts: 4.6, 7.3, 5.3 and 6.6 us, each a launch and a chain of dependent
 // reads.  (pick as the work of a row's last block instead: the fence that shows it the
-// others' sums writes back the L2 for every block, 106 us against 97 for the 64 rows.)
+// others' sums writes back the L2 for every block: 106 us in all, 97 as it was, 92 now.)
 #include <algorithm>
 
 #include "common.hpp"
@@ -163,16 +164,14 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   c.load(row_of<T>(a, b, row), lo, hi);
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    c.x[i] = logit(c.x[i]);
-    top = fmaxf(top, c.x[i]);
-  }
+  for (int i = 0; i < E; ++i) top = __builtin_amdgcn_fmed3f(c.x[i], top, INFINITY);   // (not of a NaN)
+  top = logit(top);
   // least place of the thread's largest logit (T = 0): its places grow with i
   int64_t at = lo;
   if (a.greedy && top > -INFINITY) {
 #pragma unroll
     for (int i = E - 1; i >= 0; --i)
-      if (c.x[i] == top) at = c.place(i / c.N) + i % c.N;
+      if (logit(c.x[i]) == top) at = c.place(i / c.N) + i % c.N;
   }
 #pragma unroll
   for (int m = 32; m; m >>= 1) {
@@ -200,7 +199,8 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   if (!a.greedy && top > -INFINITY) {
     const float c32 = (float)a.c;
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum += fast_exp2((c.x[i] - top) * c32);
+    for (int i = 0; i < E; ++i)
+      sum += fast_exp2(__builtin_amdgcn_fmed3f(c.x[i] - top, -3.402823466e38f, 0.0f) * c32);
 #pragma unroll
     for (int m = 32; m; m >>= 1) sum += __shfl_xor(sum, m, 64);
   }
