@@ -31,9 +31,10 @@
 // 64 rows of up to 7 drafts, 128256 tokens, bf16: stats read 214 MB in 46 us, 4.6 TB/s, bound
 // by memory (51 with each logit cleaned by itself instead of held to [-max, 0] after the
 // difference); decide 18.9 us and weigh 19.2, bound by their 20 vector instructions a share;
-// pick 7.8.  2 rows of 3 drafts: 4.6, 7.3, 5.3 and 6.6 us, each a launch and a chain of dependent
+// pick 7.8.  2 rows of 3 drafts: 4.3, 6.2, 4.8 and 6.8 us, each a launch and a chain of dependent
 // reads.  (pick as the work of a row's last block instead: the fence that shows it the
-// others' sums writes back the L2 for every block: 106 us in all, 97 as it was, 92 now.)
+// others' sums writes back the L2 for every block, 106 us in all against 97; with sums that pass
+// the L2 instead, 92 and 92, and 19.2 against 18.5 for 16 rows without draft logits.)
 #include <algorithm>
 
 #include "common.hpp"
@@ -305,15 +306,29 @@ __global__ __launch_bounds__(256) void verify_decide_kernel(VerifyArgs a) {
     const int64_t i = ((int64_t)b * a.rows + row) * a.chunks;
     float top = -INFINITY, z = 0.0f;   // z relative to the lane's top
     int32_t at = INT32_MAX;
-    for (int c = l16; c < a.chunks; c += 16) {
-      const float t = a.tops[i + c], s = a.sums[i + c];
-      if (t == -INFINITY) continue;
-      if (t > top) {
-        z = z * fast_exp2((top - t) * c32) + s;
-        top = t;
-        at = a.args[i + c];
-      } else {
-        z += s * fast_exp2((t - top) * c32);
+    for (int c0 = l16; c0 < a.chunks; c0 += 64) {   // four reads in flight
+      float ts[4], ss[4];
+      int32_t as[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = c0 + 16 * j < a.chunks;
+        const int c = in ? c0 + 16 * j : c0;
+        ts[j] = a.tops[i + c];
+        ss[j] = a.sums[i + c];
+        as[j] = a.args[i + c];
+        ts[j] = in ? ts[j] : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float t = ts[j];
+        if (t == -INFINITY) continue;
+        if (t > top) {
+          z = z * fast_exp2((top - t) * c32) + ss[j];
+          top = t;
+          at = as[j];
+        } else {
+          z += ss[j] * fast_exp2((t - top) * c32);
+        }
       }
     }
     float all = top;
