@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
   const E* vp = reinterpret_cast<const E*>(a.vp) + hk * page_elems;
   const int32_t* table = a.table + (int64_t)b * a.t_sb;
   const bool wide = a.D % 16 == 0;               // K rows are whole 16-byte chunks
-  float m = kNegBig, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float m = kLowest, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
   for (int k0 = lo + 64 * wave; k0 < hi; k0 += 256) {
     const int key = k0 + lane;
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
     ml_s[wave][1] = l;
   }
   __syncthreads();
-  float M = kNegBig, L = 0.0f, w[4];
+  float M = kLowest, L = 0.0f, w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) M = fmaxf(M, ml_s[i][0]);
 #pragma unroll
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
   const int64_t row = blockIdx.x;
   const float* ml = a.part_ml + 2 * row * a.splits;
   const float* pa = a.part_acc + row * a.splits * a.D;
-  float M = kNegBig;
+  float M = kLowest;
   for (int i = lane; i < a.splits; i += 64) M = fmaxf(M, ml[2 * i]);
 #pragma unroll
   for (int i = 32; i; i >>= 1) M = fmaxf(M, __shfl_xor(M, i, 64));

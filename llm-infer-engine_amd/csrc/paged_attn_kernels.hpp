@@ -43,6 +43,10 @@ int64_t paged_mfma_workspace(const PagedPlan& plan, int64_t n_kv_heads, int64_t 
 void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32_t dtype, bool e8,
                             hipStream_t st);
 
+// The maximum of no scores: the lowest float, so that every finite score is above it or equal,
+// and not -inf, whose difference from a masked score would be a NaN.
+constexpr float kLowest = -3.402823466e38f;
+
 // Row b's keys as its query tokens see them: token s sees keys [0, vis(s)).
 struct RowKeys {
   int64_t base;   // keys before the row's first query token

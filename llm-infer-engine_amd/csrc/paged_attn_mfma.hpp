@@ -199,6 +199,7 @@ struct PagedWave {
   Q8 q[R][G::NJ];
   f32x4 o[R][D / 16];
   float m[R], l[R];
+  bool huge;                  // a score beyond 2^26 was seen
   int vis[R];
 
   // the page of CK keys from `key` on (read as it is: checked by load)
@@ -412,11 +413,27 @@ struct PagedWave {
       // every step 47.3; 8192 keys 78.1 and 80.6)
       const bool over = top > m[rt] + 8.0f;
       if (__any(over)) {
-        const float alpha = over ? fast_exp2(m[rt] - top) : 1.0f;
+        // Beyond 2^26 a score's rounding (2^-24 of it) passes the 2^2 that p's types bear: the
+        // maximum is then taken below that, and p held to 1.
+        const bool far = fabsf(top) > 67108864.0f;
+        const float lower = fmaxf(top - fabsf(top) * 2.3841858e-07f, kLowest);
+        const float m_new = over ? (far ? lower : top) : m[rt];
+        huge |= __any(over && far) != 0;
+        const float alpha = fast_exp2(m[rt] - m_new);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[rt][i] *= alpha;
         l[rt] *= alpha;
-        m[rt] = over ? top : m[rt];
+        m[rt] = m_new;
+      }
+      float scale = c, sub = m[rt];
+      if (huge) {
+#pragma unroll
+        for (int e = 0; e < G::CK; ++e) {
+          const float x = fmaf(s[rt][e >> 2][e & 3], c, -m[rt]);
+          s[rt][e >> 2][e & 3] = x > 0.0f ? 0.0f : x;   // (a NaN stays)
+        }
+        scale = 1.0f;
+        sub = 0.0f;
       }
       float sum = 0.0f;
 #pragma unroll
@@ -424,7 +441,7 @@ struct PagedWave {
         if constexpr (G::F32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            hi[rt][u][e] = fast_exp2(fmaf(s[rt][u][e], c, -m[rt]));
+            hi[rt][u][e] = fast_exp2(fmaf(s[rt][u][e], scale, -sub));
             sum += hi[rt][u][e];
           }
         } else {
@@ -432,8 +449,8 @@ struct PagedWave {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = 8 * u + 2 * e;
-            const float p0 = fast_exp2(fmaf(s[rt][k >> 2][k & 3], c, -m[rt]));
-            const float p1 = fast_exp2(fmaf(s[rt][k >> 2][(k & 3) + 1], c, -m[rt]));
+            const float p0 = fast_exp2(fmaf(s[rt][k >> 2][k & 3], scale, -sub));
+            const float p1 = fast_exp2(fmaf(s[rt][k >> 2][(k & 3) + 1], scale, -sub));
             sum += p0 + p1;
             float h0, h1;
             h[e] = MatOp<PT>::pack(p0, p1, h0, h1);
@@ -691,6 +708,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
     w.minvis = rk.vis(list.s_first);
     w.minvis = w.minvis > w.lo ? w.minvis : w.lo;
     w.table = a.table + (int64_t)b * a.t_sb;
+    w.huge = false;
     // page numbers first: they are on their way while q is loaded
     constexpr int kStride = 4 * G::STEP;
     int base = w.lo + wave * G::STEP;
@@ -701,7 +719,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
       const int s = row / a.group, hg = row - s * a.group;
       const bool real = row < n_rows;
       w.vis[rt] = real ? rk.vis(s) : 0;
-      w.m[rt] = kNegBig;
+      w.m[rt] = kLowest;
       w.l[rt] = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) w.o[rt][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -770,7 +788,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
       w.l[rt] += swap16(w.l[rt], lane);
       w.l[rt] += swap32(w.l[rt], lane);
       if (w.vis[rt] == 0) {   // no query token (whole steps do not look at each row's keys)
-        w.m[rt] = kNegBig;
+        w.m[rt] = kLowest;
         w.l[rt] = 0.0f;
       }
       const int at = wave * kRows + 16 * rt + w.r;
@@ -787,7 +805,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_mfma_kernel(P
     for (int it = tid; it < kRows * (D / 4); it += 256) {
       const int rr = it / (D / 4), d = 4 * (it % (D / 4));
       if (row0 + rr >= n_rows) continue;
-      float M = kNegBig, L = 0.0f;
+      float M = kLowest, L = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) M = fmaxf(M, ml_s[2 * (i * kRows + rr)]);
       f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -864,7 +882,7 @@ __global__ __launch_bounds__(256) void paged_mfma_join_kernel(PagedAttnArgs a) {
   for (int rr = blockIdx.y + (share ? 0 : (int)gridDim.y * grp); rr < rows;
        rr += (int)gridDim.y * (share ? 1 : kGroups)) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    float L = 0.0f, M = kNegBig;
+    float L = 0.0f, M = kLowest;
     for (int i = i0 + (share ? lane : 0); i <= i1; i += share ? 64 : 1)
       M = fmaxf(M, a.part_ml[2 * (part_at(a, hk, tile, i, i == i0 ? end0 : 0) + rr)]);
     if (share) {

@@ -497,6 +497,43 @@ def test_attend_pages_of_extreme_scales(dev, exp):
         check_attend(dev, q, k, v, s, table, lens, dtype=BF16)
 
 
+@pytest.mark.parametrize("dtype,store,D", [(BF16, "same", 64), (F16, "e4m3", 128), (F32, "same", 128), (BF16, "e4m3", 80)])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_attend_scores_of_any_size(dev, dtype, store, D, splits, sign):
+    """All scores are finite, between 1e19 and 1e37 in size: one key (the first of the negative, the
+    last of the positive) has the largest, by so much that it has all the weight."""
+    from src.paged import paged_flash_attention
+    P, L = 16, 600
+    n = (L + P - 1) // P
+    k, v, sc = make_pages(n, 1, P, D, dtype, store, 128)
+    size = 30000.0 if dtype == F16 else 1e17
+    at = torch.arange(n * P, dtype=torch.float32).view(n, 1, P)
+    k = torch.zeros(k.shape)
+    if store == "same":
+        k[..., 0] = sign * torch.where(at == (0 if sign < 0 else L - 1), 0.5 if sign < 0 else 2000.0, 1.0 + at) \
+            * (size / 1000)
+        k = k.to(dtype)
+    else:
+        k[..., 0] = sign * torch.where(at == (0 if sign < 0 else L - 1), 0.5 if sign < 0 else 4.0, 1.0)
+        sc[..., 0] = 2.0 ** 45
+        k = k.to(E4M3)
+    q = torch.zeros(1, 2, 1, D)
+    q[..., 0] = size
+    sm_scale = 1e5 if dtype == F16 else 1.0
+    out, lse = paged_flash_attention(q.to(dtype).to(dev), cache_of(dev, k, v, sc, dtype), 0,
+                                     torch.arange(n, dtype=torch.int32, device=dev)[None],
+                                     torch.tensor([L], device=dev), sm_scale=sm_scale,
+                                     return_lse=True, num_splits=splits)
+    key = 0 if sign < 0 else L - 1
+    page, off = key // P, key % P
+    want = v[page, 0, :, off].double() * (1.0 if sc is None else float(sc[page, 0, 1]))
+    assert torch.equal(out[0, :, 0].cpu(), want.to(dtype).expand(2, D))
+    score = float(q.to(dtype)[0, 0, 0, 0]) * float(k[page, 0, off, 0]) * sm_scale
+    score *= 1.0 if sc is None else float(sc[page, 0, 0])
+    assert score * sign > 1e19 and float(((lse.double().cpu() - score) / score).abs().max()) < 1e-6
+
+
 def test_attend_rows_share_pages(dev):
     """Rows with the same first pages (a shared prefix), and a page twice in one row."""
     k, v, sc = make_pages(8, 2, 16, 128, F16, "e4m3", 113)
