@@ -273,7 +273,10 @@ extern "C" int64_t mi_paged_attn_splits(int64_t batch, int64_t n_heads, int64_t 
     return 1;
   const int64_t units = (slots * page_size + 63) / 64;
   const PagedPlan plan = paged_plan(batch, n_heads, n_kv_heads, seq_len, head_dim, dtype, 1);
-  if (plan.mfma) return paged_mfma_splits(plan, batch, n_kv_heads, head_dim, units, store);
+  if (plan.mfma) {
+    const int64_t entry = store == MI_STORE_E4M3 ? 1 : dtype == MI_DTYPE_F32 ? 4 : 2;
+    return paged_mfma_splits(plan, batch, n_kv_heads, head_dim, units, entry);
+  }
   const int64_t blocks = batch * n_heads * seq_len;
   // 8 blocks of 4 waves a compute unit, of 4 units of 64 keys or more each; a multiple of the
   // 8 L2s, so that the heads of a group, which read the same keys, find them in one (1 row of

@@ -38,7 +38,7 @@ struct PagedPlan {
 PagedPlan paged_plan(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t seq_len,
                      int64_t head_dim, int32_t dtype, int64_t num_splits);
 int64_t paged_mfma_splits(const PagedPlan& plan, int64_t batch, int64_t n_kv_heads,
-                          int64_t head_dim, int64_t units, int32_t store);
+                          int64_t head_dim, int64_t units, int64_t entry_bytes);
 int64_t paged_mfma_workspace(const PagedPlan& plan, int64_t n_kv_heads, int64_t head_dim);
 void paged_attn_mfma_launch(const PagedAttnArgs& a, const PagedPlan& plan, int32_t dtype, bool e8,
                             hipStream_t st);

@@ -19,16 +19,20 @@ PagedPlan paged_plan(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t
 }
 
 int64_t paged_mfma_splits(const PagedPlan& plan, int64_t batch, int64_t n_kv_heads,
-                          int64_t head_dim, int64_t units, int32_t store) {
+                          int64_t head_dim, int64_t units, int64_t entry_bytes) {
   // blocks of 4 waves that are resident at once, by their registers (of a CU's 3, 2 and 1; one
   // more each, in us: 64 rows of up to 4096 keys, head_dim 64, 39.0, 46.2 with 4; 64 rows of up
   // to 8192, 128, 123.0, 136.3 with 3; 1 row of 60000, 256, 54.7, 60.6 with 2)
   const int64_t fill = (head_dim == 64 && plan.r == 1 ? 3 : head_dim == 256 ? 1 : 2) *
                        (int64_t)device_cu_count();
   const int64_t blocks = n_kv_heads * plan.tiles;
-  // a block a row, and one launch, where no row has more than 16 units of keys (8 rows of up
-  // to 1000 keys: head_dim 64 10.2 us, divided 14.7; 128 15.3 and 17.5)
-  if (units <= 16) return 1;
+  // a block a row, and one launch, where no row has more than 16 units of keys, or 32 of 64
+  // bytes (us, calls among others, undivided and divided; 2000 8-bit keys of 64 dims: 1 row
+  // 12.3 and 16.2, 16 rows 11.2 and 15.9, 64 rows 19.3 and 26.2, 3000 keys 16.8 and 16.0, 17.7
+  // and 17.6, 27.0 and 31.2; bf16 keys of 128 dims, 800: 17.0 and 15.8, 17.5 and 22.1, 31.8 and
+  // 35.5, 1500: 25.8 and 16.5, 27.1 and 22.8, 52.4 and 43.7)
+  const int64_t most_units = head_dim * entry_bytes <= 64 ? 32 : 16;
+  if (units <= most_units) return 1;
   int64_t parts = fill / blocks;
   const int64_t most = batch * ((units + 3) / 4);
   if (parts > most) parts = most;
