@@ -3,7 +3,7 @@
 //
 // A wave holds R tiles of 16 query rows of one KV head (row = token * group + head of
 // the group) and streams its keys from memory straight into matrix operands: nothing
-// passes through LDS until the end.  Per step of 64 keys (8-bit pages) or 32:
+// passes through LDS until the end.  Per step of 64 keys (8-bit pages), 32 or (fp32) 16:
 //   S^T = K Q^T      v_mfma_f32_16x16x32: A = 16 keys x 32 dims, B = 32 dims x 16 rows.
 //                    A lane's operand is 8 dims of one key; the order of the dims is
 //                    free as long as Q has the same, so each lane takes whole 16-byte
@@ -17,7 +17,7 @@
 //                    needs 8 keys of row r: those it already has (no shuffle), and
 //                    V^T's lane the same 8 keys of one dim: 8 or 16 neighbouring entries
 //                    of the transposed V page, one 16-byte load.
-// 8-bit entries become bf16 (K: q's type) two at a time with v_cvt_scalef32_pk, exactly;
+// 8-bit entries become bf16 (K, and with fp32 queries V: q's type) two at a time with v_cvt_scalef32_pk, exactly;
 // V's page scale is the instruction's scale operand (bf16 has fp32's range, so no page
 // overflows), K's multiplies the scores.  p goes in as a 16-bit value and its remainder
 // (two products): off by 2^-16 at most, where one rounding of p to q's type would add an
